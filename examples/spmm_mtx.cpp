@@ -117,7 +117,7 @@ int main(int argc, char **argv) {
     const size_t sb = dgs_spmm_hub_selftest_bytes();
     HIP_OK(hipMalloc(&d_st, sb));
     const int v = dgs_spmm_hub_selftest(d_st, sb, st);
-    printf("hub-chain self-test on this device: %s\n", v == 1 ? "passed" : (v == 0 ? "FAILED (chains off)" : dgs_strerror(v)));
+    printf("hub chains on this device (self-test): %s\n", v == 1 ? "on" : (v == 0 ? "FAILED (chains off)" : dgs_strerror(v)));
     HIP_OK(hipFree(d_st));
   }
   int maxlen = 0;
