@@ -1,0 +1,490 @@
+// embedding.hip -- embedding lookup with scaling, and the table's gradient by sorted tokens.
+//
+//   out[p, :] = scale * table[ids[p], :]              a negative id is "no token": a row of zeros; an id >= V gives a row of NaN (nothing is
+//                                                     read out of bounds, and the mistake is seen)
+//   dtable[v, :] = scale * sum over p with ids[p] = v, in the order of p, of dout[p, :]       (ids that are negative, >= V or equal to the
+//                                                     padding id add to no row; a row without a token is 0)
+//
+// Lookup: HBM-bound gather, each row read once in 16-byte pieces.
+// Gradient: positions are sorted by id with the position as the tie-break (dgs_embedding_sort_*), so every row's sum has one fixed order
+// and no atomics.  The sorted list is cut into chunks of `chunk` positions; a group of lanes walks a chunk with a running sum in 32 bits
+// and writes each row that lies within its chunk.  A row whose positions cross a chunk's border (a frequent token) leaves partial sums in the
+// workspace, which embedding_join adds up in chunk order.  Rows without a token are cleared by workgroups of the same launch: they find
+// the few ids of their share of the table by binary search in the sorted list, so the table is written once and read never.
+#include "dense_common.h"
+
+namespace dgs {
+
+constexpr int kSortSmall = 4096;   // positions up to here: one launch that counts ranks
+constexpr int kSortWaves = 8;      // waves of a radix-sort workgroup
+constexpr int kSortBits = 9;       // at most this many bits a pass (512 bins)
+constexpr int kSortBlocks = 256;   // at most this many workgroups a pass (each reads all the others' counts)
+
+template <typename I>
+__device__ __forceinline__ uint32_t token_key(I id, int64_t V, int64_t pad) {
+  const int64_t v = (int64_t)id;
+  return v < 0 || v >= V || v == pad ? (uint32_t)V : (uint32_t)v;  // V: adds to no row, sorted behind all others
+}
+
+// ---- lookup ----------------------------------------------------------------------------------------------------------------
+// G lanes a row (a power of two <= 256), kBlock / G rows a workgroup.
+template <typename T, typename I, bool VECTOR>
+__global__ __launch_bounds__(kBlock) void embedding_fwd_kernel(int64_t n, int64_t V, int D, int G, const I *__restrict__ ids,
+                                                               const T *__restrict__ table, int64_t ld, float scale, T *__restrict__ out) {
+  constexpr int W = kVec<T>;
+  const int lane = threadIdx.x & (G - 1);
+  const int64_t p = (int64_t)blockIdx.x * (kBlock / G) + threadIdx.x / G;
+  if (p >= n) return;
+  const int64_t id = (int64_t)ids[p];
+  const bool there = id >= 0 && id < V;
+  const T *row = table + (there ? id : 0) * ld;
+  const float none = id < 0 ? 0.0f : __builtin_nanf("");
+  for (int c = lane * W; c < D; c += G * W) {
+    float x[W];
+    if (there) {
+      load_row<T, VECTOR>(row, c, D, x);
+#pragma unroll
+      for (int k = 0; k < W; k++) x[k] *= scale;
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; k++) x[k] = none;
+    }
+    store_row<T, VECTOR>(out + p * (int64_t)D, c, D, x);
+  }
+}
+
+// ---- sorting ---------------------------------------------------------------------------------------------------------------
+// Few positions: the place of (key, p) in the sorted list is the number of pairs in front of it.  A workgroup ranks 32 positions, 8
+// threads each an eighth of the list out of LDS; no pass waits for another.
+template <typename I>
+__global__ __launch_bounds__(kBlock) void embedding_rank_kernel(int n, int64_t V, int64_t pad, const I *__restrict__ ids,
+                                                                uint32_t *__restrict__ skey, int *__restrict__ spos) {
+  __shared__ uint32_t key[kSortSmall];
+  __shared__ int part[8][32];
+  for (int p = threadIdx.x; p < n; p += kBlock) key[p] = token_key(ids[p], V, pad);
+  __syncthreads();
+  const int mine = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int p = blockIdx.x * 32 + mine;
+  int before = 0;
+  const uint32_t k = p < n ? key[p] : 0u;
+  const int len = (n + 7) / 8, lo = sub * len, hi = lo + len < n ? lo + len : n;
+  for (int o = lo; o < hi; o++) before += key[o] < k || (key[o] == k && o < p);
+  part[sub][mine] = before;
+  __syncthreads();
+  if (sub == 0 && p < n) {
+    int at = 0;
+#pragma unroll
+    for (int s = 0; s < 8; s++) at += part[s][mine];
+    skey[at] = k;
+    spos[at] = p;
+  }
+}
+
+// Many positions: a stable radix sort from the low digit, two launches a pass (counts, then placement), `tile` positions a workgroup.
+template <typename I>
+__global__ __launch_bounds__(kSortWaves *kWave) void embedding_count_kernel(int64_t n, int64_t V, int64_t pad, int tile, int shift, int bits,
+                                                                            const I *__restrict__ ids, const uint32_t *__restrict__ kin,
+                                                                            int *__restrict__ hist) {
+  __shared__ int cnt[1 << kSortBits];
+  const int bins = 1 << bits;
+  for (int b = threadIdx.x; b < bins; b += blockDim.x) cnt[b] = 0;
+  __syncthreads();
+  const int64_t lo = (int64_t)blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n;
+  for (int64_t p = lo + threadIdx.x; p < hi; p += blockDim.x) {
+    const uint32_t k = kin ? kin[p] : token_key(ids[p], V, pad);
+    atomicAdd(&cnt[(k >> shift) & (bins - 1)], 1);  // (a count: its order changes nothing)
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += blockDim.x) hist[(int64_t)blockIdx.x * bins + b] = cnt[b];
+}
+
+template <typename I>
+__global__ __launch_bounds__(kSortWaves *kWave) void embedding_place_kernel(int64_t n, int64_t V, int64_t pad, int tile, int shift, int bits,
+                                                                            const I *__restrict__ ids, const uint32_t *__restrict__ kin,
+                                                                            const int *__restrict__ pin, const int *__restrict__ hist,
+                                                                            uint32_t *__restrict__ kout, int *__restrict__ pout) {
+  __shared__ int off[kSortWaves][1 << kSortBits];  // next place of a digit for each wave's part of the tile
+  __shared__ int wsum[kSortWaves];
+  static_assert((1 << kSortBits) <= kSortWaves * kWave, "a thread for each bin");
+  const int bins = 1 << bits, t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+  const int64_t lo = (int64_t)blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n;
+  const int share = tile / kSortWaves;  // (a multiple of 64)
+  const int64_t wlo = lo + (int64_t)wave * share, whi = wlo + share < hi ? wlo + share : hi;
+  for (int b = t; b < kSortWaves << kSortBits; b += blockDim.x) off[b >> kSortBits][b & ((1 << kSortBits) - 1)] = 0;
+  __syncthreads();
+  for (int64_t p = wlo + lane; p < whi; p += kWave) {
+    const uint32_t k = kin ? kin[p] : token_key(ids[p], V, pad);
+    atomicAdd(&off[wave][(k >> shift) & (bins - 1)], 1);
+  }
+  // this thread's digit: positions with it in all workgroups, and in those in front of this one
+  int all = 0, front = 0;
+  if (t < bins) {
+#pragma unroll 8
+    for (int b = 0; b < (int)gridDim.x; b++) {
+      const int h = hist[(int64_t)b * bins + t];
+      all += h;
+      front += b < (int)blockIdx.x ? h : 0;
+    }
+  }
+  int scan = all;  // inclusive over the digits: in the wave, then over the waves
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int o = __shfl_up(scan, d, 64);
+    if (lane >= d) scan += o;
+  }
+  if (lane == kWave - 1) wsum[wave] = scan;
+  __syncthreads();
+  if (t < bins) {
+    int base = scan - all + front;
+    for (int w = 0; w < wave; w++) base += wsum[w];
+    for (int w = 0; w < kSortWaves; w++) {  // the waves' parts follow each other
+      const int c = off[w][t];
+      off[w][t] = base;
+      base += c;
+    }
+  }
+  __syncthreads();
+  // placement: each wave goes through its part 64 positions at a time; lanes with the same digit rank among themselves by ballots.  Only
+  // this wave touches off[wave]; its LDS accesses are kept in program order by the wave barriers.
+  for (int64_t p0 = wlo; p0 < whi; p0 += kWave) {
+    const int64_t p = p0 + lane;
+    const bool on = p < whi;
+    const uint32_t k = on ? (kin ? kin[p] : token_key(ids[p], V, pad)) : 0u;
+    const int digit = (int)((k >> shift) & (bins - 1));
+    uint64_t peers = __ballot(on);
+    for (int b = 0; b < bits; b++) {
+      const uint64_t set = __ballot((digit >> b) & 1);
+      peers &= (digit >> b) & 1 ? set : ~set;
+    }
+    const int rank = __popcll(peers & ((1ull << lane) - 1));
+    int at = 0;
+    if (on) at = off[wave][digit] + rank;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (on && rank == 0) off[wave][digit] = at + __popcll(peers);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (on) {
+      kout[at] = k;
+      pout[at] = pin ? pin[p] : (int)p;
+    }
+  }
+}
+
+// ---- gradient --------------------------------------------------------------------------------------------------------------
+// Workgroups [0, fill_blocks): rows without a token.  The others: chunks of the sorted list.  Partial rows: slot 2c for the row that
+// chunk c goes on with from the chunk before, slot 2c + 1 for the row that starts in chunk c and goes on behind it.
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_t V, int D, int G, int chunk, int64_t n_chunks, int64_t fill_blocks, int fill_rows,
+                                                               const uint32_t *__restrict__ skey, const int *__restrict__ spos,
+                                                               const T *__restrict__ dout, int64_t ldo, float scale, T *__restrict__ dtable,
+                                                               float *__restrict__ partial) {
+  constexpr int W = kVec<T>;
+  if ((int64_t)blockIdx.x < fill_blocks) {
+    // fill_rows (<= 256) rows from v0.  The sorted list's part with these ids lies between two lower bounds; a wave looks for each by
+    // 64-fold splitting: 3 steps for 2^18 positions.
+    __shared__ uint32_t seen[8];
+    __shared__ int64_t bound[2];
+    const int64_t v0 = (int64_t)blockIdx.x * fill_rows, v1 = v0 + fill_rows < V ? v0 + fill_rows : V;
+    const int t = threadIdx.x;
+    if (t < 8) seen[t] = 0u;
+    if (t < 2 * kWave) {
+      const int lane = t & 63;
+      const uint32_t key = (uint32_t)(t < kWave ? v0 : v1);
+      int64_t lo = 0, hi = n;  // the answer lies in [lo, hi]
+      while (hi > lo) {
+        const int64_t step = (hi - lo + kWave - 1) / kWave;
+        const int64_t at = lo + lane * step;
+        const int less = __popcll(__ballot(at < hi && skey[at < hi ? at : lo] < key));  // probes in front of the bound: the first `less` lanes
+        const int64_t nlo = less ? lo + (int64_t)(less - 1) * step + 1 : lo;
+        const int64_t nhi = lo + (int64_t)less * step;
+        hi = nhi < hi ? nhi : hi;
+        lo = nlo;
+      }
+      if (lane == 0) bound[t / kWave] = lo;
+    }
+    __syncthreads();
+    for (int64_t q = bound[0] + t; q < bound[1]; q += kBlock) {
+      const int r = (int)((int64_t)skey[q] - v0);
+      atomicOr(&seen[r >> 5], 1u << (r & 31));
+    }
+    __syncthreads();
+    float zero[W];
+#pragma unroll
+    for (int k = 0; k < W; k++) zero[k] = 0.0f;
+    const int lane = t & (G - 1);
+    for (int64_t v = v0 + t / G; v < v1; v += kBlock / G) {
+      const int r = (int)(v - v0);
+      if ((seen[r >> 5] >> (r & 31)) & 1) continue;
+      for (int c = lane * W; c < D; c += G * W) store_row_stream<T, VECTOR>(dtable + v * (int64_t)D, c, D, zero);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & (G - 1);
+  const int64_t ch = ((int64_t)blockIdx.x - fill_blocks) * (kBlock / G) + threadIdx.x / G;
+  if (ch >= n_chunks) return;
+  const int64_t q0 = ch * chunk, q1 = q0 + chunk < n ? q0 + chunk : n;
+  const int c = ((int)blockIdx.y * G + lane) * W;
+  if (c >= D) return;
+  bool head = ch > 0 && skey[q0 - 1] == skey[q0];  // the first row goes on from the chunk before
+  float acc[W];
+#pragma unroll
+  for (int k = 0; k < W; k++) acc[k] = 0.0f;
+  uint32_t key = skey[q0];
+  constexpr int U = 4;  // rows in flight
+  for (int64_t q = q0; q < q1; q += U) {
+    float x[U][W];
+    uint32_t kk[U + 1];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int64_t at = q + u < q1 ? q + u : q1 - 1;
+      kk[u] = skey[at];
+      if (kk[u] < (uint32_t)V) load_row<T, VECTOR>(dout + (int64_t)spos[at] * ldo, c, D, x[u]);
+    }
+    kk[U] = q + U < n ? skey[q + U] : 0xffffffffu;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (q + u >= q1 || kk[u] >= (uint32_t)V) break;
+      key = kk[u];
+#pragma unroll
+      for (int k = 0; k < W; k++) acc[k] += x[u][k];
+      const bool last = q + u + 1 >= q1;                                     // of the chunk
+      const uint32_t next = last ? (q1 < n ? skey[q1] : 0xffffffffu) : kk[u + 1];
+      if (next != key || last) {
+        const bool on = next == key;  // the row goes on in the next chunk
+        if (head || on) {
+          float *slot = partial + (2 * ch + (head ? 0 : 1)) * (int64_t)D;
+#pragma unroll
+          for (int k = 0; k < W; k++)
+            if (c + k < D) slot[c + k] = acc[k];
+        } else {
+#pragma unroll
+          for (int k = 0; k < W; k++) acc[k] *= scale;
+          store_row<T, VECTOR>(dtable + (int64_t)key * D, c, D, acc);
+        }
+        head = false;
+#pragma unroll
+        for (int k = 0; k < W; k++) acc[k] = 0.0f;
+      }
+    }
+  }
+}
+
+// Border b between chunks b - 1 and b: the workgroups of the row that starts in chunk b - 1 and goes on in chunk b add up its partial
+// sums: the start's, then one of each chunk up to the last.  32 columns x 8 shares of the chunks; the shares' sums are joined in order.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void embedding_join_kernel(int64_t n, int64_t V, int D, int chunk, int64_t n_chunks, const uint32_t *__restrict__ skey,
+                                                                float scale, const float *__restrict__ partial, T *__restrict__ dtable) {
+  const int64_t b = (int64_t)blockIdx.x + 1;
+  const int64_t at = b * chunk;
+  const uint32_t key = skey[at];
+  if (key >= (uint32_t)V || skey[at - 1] != key) return;
+  if (b > 1 && skey[at - chunk - 1] == key) return;  // an earlier border owns the row
+  __shared__ int64_t end;
+  __shared__ float sum[8][32];
+  if (threadIdx.x == 0) {  // the last chunk that begins within the row: binary search over the chunks' first keys
+    int64_t lo = b, hi = n_chunks - 1;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi + 1) / 2;
+      if (skey[mid * chunk] == key) lo = mid; else hi = mid - 1;
+    }
+    end = lo;
+  }
+  __syncthreads();
+  const int col = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int64_t m = end - b + 1, len = (m + 7) / 8;  // chunks b .. end, an eighth each
+  const int64_t lo = b + sub * len, hi = lo + len < end + 1 ? lo + len : end + 1;
+  for (int c0 = (int)blockIdx.y * 32; c0 < D; c0 += (int)gridDim.y * 32) {
+    const int c = c0 + col;
+    float a = 0.0f;
+    if (c < D) {
+      if (sub == 0) a = partial[(2 * (b - 1) + 1) * (int64_t)D + c];
+      int64_t k = lo;
+      for (; k + 3 < hi; k += 4) {
+        const float p0 = partial[2 * k * (int64_t)D + c], p1 = partial[2 * (k + 1) * (int64_t)D + c], p2 = partial[2 * (k + 2) * (int64_t)D + c],
+                    p3 = partial[2 * (k + 3) * (int64_t)D + c];
+        a += (p0 + p1) + (p2 + p3);
+      }
+      for (; k < hi; k++) a += partial[2 * k * (int64_t)D + c];
+    }
+    sum[sub][col] = a;
+    __syncthreads();
+    if (sub == 0 && c < D) {
+      float s = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; k++) s += sum[k][col];
+      dtable[(int64_t)key * D + c] = from_f32<T>(s * scale);
+    }
+    __syncthreads();
+  }
+}
+
+static int lanes_for(int64_t vecs) {
+  int G = 1;
+  while (G < vecs && G < kBlock) G <<= 1;
+  return G;
+}
+static int key_bits(int64_t V) {  // keys 0 .. V
+  int b = 1;
+  while (((int64_t)1 << b) <= V) b++;
+  return b;
+}
+// Positions a chunk: enough chunks for the card, and for very long lists few enough that a frequent token's partial sums stay few.
+static int chunk_of(int64_t n) { return n <= (1 << 20) ? 32 : 256; }
+
+struct SortPlan {
+  int passes, bits, tile;
+  int64_t blocks;
+};
+static SortPlan sort_plan(int64_t n, int64_t V) {
+  SortPlan p;
+  const int kb = key_bits(V);
+  p.passes = (kb + kSortBits - 1) / kSortBits;
+  p.bits = (kb + p.passes - 1) / p.passes;
+  const int64_t least = kSortWaves * kWave;  // 64 positions a wave
+  int64_t tile = (n + kSortBlocks - 1) / kSortBlocks;
+  tile = tile < 2 * least ? 2 * least : (tile + least - 1) / least * least;
+  p.tile = (int)tile;
+  p.blocks = (n + tile - 1) / tile;
+  return p;
+}
+struct BwdLayout { size_t key[2], pos[2], hist, partial, total; };
+static BwdLayout bwd_layout(int64_t n, int64_t V, int64_t D) {
+  BwdLayout L;
+  size_t at = 0;
+  auto take = [&](size_t bytes) { const size_t o = at; at += round_up(bytes, 256); return o; };
+  const bool small = n <= kSortSmall;
+  for (int i = 0; i < 2; i++) {
+    L.key[i] = take(i && small ? 0 : (size_t)n * 4);
+    L.pos[i] = take(i && small ? 0 : (size_t)n * 4);
+  }
+  const SortPlan p = sort_plan(n, V);
+  L.hist = take(small ? 0 : (size_t)p.blocks * (1u << p.bits) * 4);
+  const int chunk = chunk_of(n);
+  L.partial = take((size_t)((n + chunk - 1) / chunk) * 2 * D * 4);
+  L.total = at;
+  return L;
+}
+
+template <typename T, typename I>
+static int fwd(int64_t n, int64_t V, int64_t D, const void *ids, const void *table, int64_t ld, float scale, void *out, hipStream_t st) {
+  const bool vec = D % kVec<T> == 0 && ld % kVec<T> == 0 && aligned_to(table, 16) && aligned_to(out, 16);
+  const int G = lanes_for((D + kVec<T> - 1) / kVec<T>);
+  const int64_t blocks = (n + kBlock / G - 1) / (kBlock / G);
+  if (vec)
+    hipLaunchKernelGGL((embedding_fwd_kernel<T, I, true>), dim3((unsigned)blocks), dim3(kBlock), 0, st, n, V, (int)D, G, (const I *)ids, (const T *)table, ld, scale, (T *)out);
+  else
+    hipLaunchKernelGGL((embedding_fwd_kernel<T, I, false>), dim3((unsigned)blocks), dim3(kBlock), 0, st, n, V, (int)D, G, (const I *)ids, (const T *)table, ld, scale, (T *)out);
+  return check_launch();
+}
+
+template <typename I>
+static int sort_ids(int64_t n, int64_t V, int64_t pad, const I *ids, char *ws, const BwdLayout &L, uint32_t **key, int **pos, hipStream_t st) {
+  if (n <= kSortSmall) {
+    *key = (uint32_t *)(ws + L.key[0]);
+    *pos = (int *)(ws + L.pos[0]);
+    hipLaunchKernelGGL((embedding_rank_kernel<I>), dim3((unsigned)((n + 31) / 32)), dim3(kBlock), 0, st, (int)n, V, pad, ids, *key, *pos);
+    return check_launch();
+  }
+  const SortPlan p = sort_plan(n, V);
+  int *hist = (int *)(ws + L.hist);
+  const uint32_t *kin = nullptr;
+  const int *pin = nullptr;
+  for (int i = 0; i < p.passes; i++) {
+    uint32_t *kout = (uint32_t *)(ws + L.key[i & 1]);
+    int *pout = (int *)(ws + L.pos[i & 1]);
+    const dim3 grid((unsigned)p.blocks), block(kSortWaves * kWave);
+    hipLaunchKernelGGL((embedding_count_kernel<I>), grid, block, 0, st, n, V, pad, p.tile, i * p.bits, p.bits, ids, kin, hist);
+    hipLaunchKernelGGL((embedding_place_kernel<I>), grid, block, 0, st, n, V, pad, p.tile, i * p.bits, p.bits, ids, kin, pin, hist, kout, pout);
+    if (check_launch() != DGS_OK) return DGS_ELAUNCH;
+    kin = kout;
+    pin = pout;
+    *key = kout;
+    *pos = pout;
+  }
+  return DGS_OK;
+}
+
+template <typename T>
+static int bwd(int64_t n, int64_t V, int64_t D, const uint32_t *key, const int *pos, const void *dout, int64_t ldo, float scale, void *dtable, float *partial,
+               hipStream_t st) {
+  const bool vec = D % kVec<T> == 0 && ldo % kVec<T> == 0 && aligned_to(dout, 16) && aligned_to(dtable, 16);
+  const int64_t vecs = (D + kVec<T> - 1) / kVec<T>;
+  const int G = lanes_for(vecs), chunk = chunk_of(n);
+  const int64_t n_chunks = (n + chunk - 1) / chunk, per = kBlock / G;
+  // a clearing workgroup writes about 64 KB; its rows go by a bit map of 256
+  const int64_t rowb = D * (int64_t)sizeof(T);
+  const int fill_rows = (int)(65536 / rowb < 1 ? 1 : 65536 / rowb > 256 ? 256 : 65536 / rowb);
+  const int64_t fill = (V + fill_rows - 1) / fill_rows, work = (n_chunks + per - 1) / per;
+  if (fill + work > INT32_MAX) return DGS_ERANGE;
+  const int64_t tiles = (vecs + G - 1) / G;
+  if (tiles > 65535) return DGS_ERANGE;
+  // (the clearing part of a launch with several column tiles runs in the first of them alone)
+  for (int part = 0; part < (tiles > 1 ? 2 : 1); part++) {
+    const int64_t f = tiles > 1 && part ? 0 : fill, w = tiles > 1 && !part ? 0 : work;
+    const dim3 grid((unsigned)(f + w), (unsigned)(tiles > 1 && !part ? 1 : tiles));
+    if (vec)
+      hipLaunchKernelGGL((embedding_bwd_kernel<T, true>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, f, fill_rows, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
+    else
+      hipLaunchKernelGGL((embedding_bwd_kernel<T, false>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, f, fill_rows, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
+  }
+  if (check_launch() != DGS_OK) return DGS_ELAUNCH;
+  if (n_chunks > 1) {
+    const int64_t cols = (D + 31) / 32;
+    hipLaunchKernelGGL((embedding_join_kernel<T>), dim3((unsigned)(n_chunks - 1), (unsigned)(cols < 16 ? cols : 16)), dim3(kBlock), 0, st, n, V, (int)D, chunk, n_chunks, key, scale,
+                       partial, (T *)dtable);
+  }
+  return check_launch();
+}
+
+}  // namespace dgs
+
+using namespace dgs;
+
+static int embedding_sizes(int dtype, int id_bytes, int64_t n, int64_t V, int64_t D) {
+  if (!dtype_ok(dtype) || (id_bytes != 4 && id_bytes != 8) || n < 0 || V < 0 || D <= 0) return DGS_EINVAL;
+  if (n >= INT32_MAX || V >= INT32_MAX || D >= INT32_MAX / 64) return DGS_ERANGE;
+  return DGS_OK;
+}
+
+extern "C" int dgs_embedding(int dtype, int id_bytes, int64_t n, int64_t V, int64_t D, const void *ids, const void *table, int64_t ld_table, float scale,
+                             void *out, dgsStream_t stream) {
+  const int rc = embedding_sizes(dtype, id_bytes, n, V, D);
+  if (rc != DGS_OK) return rc;
+  if (n == 0) return DGS_OK;
+  if (!ids || !out || (V > 0 && !table)) return DGS_EINVAL;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+#define DGS_GO(T) return id_bytes == 8 ? fwd<T, int64_t>(n, V, D, ids, table, ld_table, scale, out, st) : fwd<T, int32_t>(n, V, D, ids, table, ld_table, scale, out, st)
+  if (dtype == DGS_F32) DGS_GO(float);
+  if (dtype == DGS_F16) DGS_GO(f16);
+  DGS_GO(bf16);
+#undef DGS_GO
+}
+
+extern "C" size_t dgs_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D) {
+  if (n <= 0 || V < 0 || D <= 0) return 256;
+  return bwd_layout(n, V, D).total;
+}
+
+extern "C" int dgs_embedding_bwd(int dtype, int id_bytes, int64_t n, int64_t V, int64_t D, const void *ids, int64_t padding_idx, const void *dout, int64_t ld_dout,
+                                 float scale, void *dtable, void *workspace, size_t workspace_bytes, dgsStream_t stream) {
+  const int rc = embedding_sizes(dtype, id_bytes, n, V, D);
+  if (rc != DGS_OK) return rc;
+  if (V == 0) return DGS_OK;
+  if (!dtable || (n > 0 && (!ids || !dout))) return DGS_EINVAL;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  uint32_t *key = nullptr;
+  int *pos = nullptr;
+  float *partial = nullptr;
+  if (n > 0) {
+    if (!workspace || workspace_bytes < dgs_embedding_bwd_workspace_bytes(n, V, D)) return DGS_EWORKSPACE;
+    char *ws = static_cast<char *>(workspace);
+    const BwdLayout L = bwd_layout(n, V, D);
+    partial = (float *)(ws + L.partial);
+    const int r = id_bytes == 8 ? sort_ids<int64_t>(n, V, padding_idx, (const int64_t *)ids, ws, L, &key, &pos, st)
+                                : sort_ids<int32_t>(n, V, padding_idx, (const int32_t *)ids, ws, L, &key, &pos, st);
+    if (r != DGS_OK) return r;
+  }
+  if (dtype == DGS_F32) return bwd<float>(n, V, D, key, pos, dout, ld_dout, scale, dtable, partial, st);
+  if (dtype == DGS_F16) return bwd<f16>(n, V, D, key, pos, dout, ld_dout, scale, dtable, partial, st);
+  return bwd<bf16>(n, V, D, key, pos, dout, ld_dout, scale, dtable, partial, st);
+}

@@ -1,0 +1,393 @@
+// gated_ffn.hip -- the gated feed-forward product h = act(x Wg^T) * (x Wu^T) in one kernel, with its backward pass.
+//
+//   forward    g = x Wg^T, u = x Wu^T side by side in one tile (kDual: a wave holds the g and the u of the same columns), h = act(g) u where
+//              the tile's sums leave the registers: g and u never reach memory.
+//   backward   the forward's products are made again (4 rows D F flops, instead of keeping 8 bytes for each value of h), and where they
+//              leave the registers  dg = dh u act'(g), du = dh act(g), rounded once to the type: the operands of the other products,
+//              dx = dg Wg + du Wu  (one walk over 2 F),  dWg = dg^T x, dWu = du^T x  (sums over the rows, split where there are few tiles).
+//
+// Bound: the matrix cores (12 rows D F flops forward and backward, 16 with the products made again); for few rows the weights' bytes
+// (gated_few_kernel).  Sums are held in 32 bits.
+#include "gemm_core.h"
+
+namespace dgs {
+
+// act(g) and act'(g) in 32 bits.  silu: g s, s (1 + g (1 - s)) with s = 1 / (1 + exp(-g)); gelu: g c, c + g p with the normal
+// distribution's c and density p; relu.
+template <int ACT>
+__device__ __forceinline__ float act(float g, float &d) {
+  if constexpr (ACT == DGS_ACT_RELU) {
+    d = g > 0.0f ? 1.0f : 0.0f;
+    return g < 0.0f ? 0.0f : g;  // (a NaN stays)
+  } else if constexpr (ACT == DGS_ACT_SILU) {
+    const float s = 1.0f / (1.0f + __expf(-g));
+    d = s * (1.0f + g * (1.0f - s));
+    return g * s;
+  } else {
+    const float c = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    d = c + g * (0.39894228040143268f * __expf(-0.5f * g * g));
+    return g * c;
+  }
+}
+
+struct GatedOut {
+  const void *dh;   // backward: [M, F], contiguous
+  void *o0, *o1;    // forward: h; backward: dg, du
+  int64_t F, ldo;   // columns of h / dh; row stride of the outputs (backward: the padded columns F .. ldo are written too, as zeros)
+};
+
+template <typename T, int ACT, bool BWD>
+__device__ __forceinline__ void gated_store(const GatedOut &o, int64_t m, int64_t n, const f32x4 &g, const f32x4 &u, bool vec) {
+  f32x4 a, b;
+  if constexpr (BWD) {
+    const f32x4 dh = n < o.F ? load4<T>((const T *)o.dh + m * o.F + n, o.F - n, o.F % 4 == 0) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      float d;
+      const float v = act<ACT>(g[k], d);
+      // (behind F: g = u = 0 and dh = 0 give the zeros that the padding has to hold)
+      a[k] = dh[k] * u[k] * d;
+      b[k] = dh[k] * v;
+    }
+    store4<T>((T *)o.o0 + m * o.ldo + n, a, o.ldo - n, true);
+    store4<T>((T *)o.o1 + m * o.ldo + n, b, o.ldo - n, true);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      float d;
+      a[k] = act<ACT>(g[k], d) * u[k];
+    }
+    store4<T>((T *)o.o0 + m * o.ldo + n, a, o.F - n, vec);
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int ACT, bool BWD>
+__global__ __launch_bounds__(64 * WM *WN) void gated_kernel(const GemmArgs g, const GatedOut o) {
+  using G = Gemm<T, BM, BN, WM, WN, false, false, kDual>;
+  DGS_GEMM_LDS(G)
+  const Where at = where_of(g.tiles_m, g.tiles_n);
+  const int m0 = at.m * BM, n0 = at.n * G::kCols;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, wm = wave / WN, wn = wave % WN;
+  const int steps = (int)((g.K + G::TA::kK - 1) / G::TA::kK);
+  f32x4 acc[G::FM][G::FN];
+  gemm_loop<G>(g, m0, n0, 0, steps, steps, 0, false, false, sizeof(T), ldsA0, ldsB0, ldsA1, ldsB1, wm, wn, lane, acc);
+  const bool vec = o.ldo % 4 == 0;
+  const int64_t end = BWD ? o.ldo : o.F;
+#pragma unroll
+  for (int i = 0; i < G::FM; i++) {
+    const int64_t m = m0 + wm * (BM / WM) + 16 * i + (lane & 15);
+    if (m >= g.M) continue;
+#pragma unroll
+    for (int j = 0; j < G::FN / 2; j++) {
+      const int64_t n = n0 + G::c_col(wn, j) + 4 * (lane >> 4);
+      if (n < end) gated_store<T, ACT, BWD>(o, m, n, acc[i][j], acc[i][j + G::FN / 2], vec);
+    }
+  }
+}
+
+// Few rows (<= 16 FM): 8 waves share the K of 16 columns of Wg and of Wu, whose rows go from memory to the registers of the matrix
+// instructions (128 bytes of each of 16 rows a wave at a time); x comes out of L2.  The waves' sums meet in LDS.
+template <typename T, int FM, int ACT>
+__global__ __launch_bounds__(512) void gated_few_kernel(const char *__restrict__ x, int64_t ldx, const char *__restrict__ wg, const char *__restrict__ wu, int64_t ldw,
+                                                        int M, int64_t F, int64_t kbytes, T *__restrict__ h) {
+  constexpr int kW = 8;
+  __shared__ float sum[kW][2][16 * FM][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int r = lane & 15;
+  const int64_t n = n0 + r < F ? n0 + r : F - 1;
+  const char *pg = wg + n * ldw + (lane >> 4) * 16, *pu = wu + n * ldw + (lane >> 4) * 16;
+  const char *px[FM];
+#pragma unroll
+  for (int i = 0; i < FM; i++) px[i] = x + (int64_t)(16 * i + r < M ? 16 * i + r : M - 1) * ldx + (lane >> 4) * 16;
+  f32x4 ag[FM], au[FM];
+#pragma unroll
+  for (int i = 0; i < FM; i++) ag[i] = au[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const dgs_u4 zero = {0u, 0u, 0u, 0u};
+  constexpr int U = FM == 1 ? 4 : 2;  // 128-byte steps in flight
+  for (int64_t k0 = wave * 128; k0 < kbytes; k0 += kW * 128 * U) {
+    Slice g[U][2], u[U][2], a[U][2][FM];
+#pragma unroll
+    for (int s = 0; s < U; s++)
+#pragma unroll
+      for (int kk = 0; kk < 2; kk++) {
+        const int64_t k = k0 + (int64_t)s * kW * 128 + kk * 64;
+        const bool on = k + (lane >> 4) * 16 < kbytes;
+        g[s][kk].u = on ? __builtin_nontemporal_load((const dgs_u4 *)(pg + k)) : zero;
+        u[s][kk].u = on ? __builtin_nontemporal_load((const dgs_u4 *)(pu + k)) : zero;
+#pragma unroll
+        for (int i = 0; i < FM; i++) a[s][kk][i].u = on ? *(const dgs_u4 *)(px[i] + k) : zero;
+      }
+#pragma unroll
+    for (int s = 0; s < U; s++)
+#pragma unroll
+      for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+        for (int i = 0; i < FM; i++) {
+          Mma<T>::step(ag[i], g[s][kk], a[s][kk][i]);
+          Mma<T>::step(au[i], u[s][kk], a[s][kk][i]);
+        }
+  }
+#pragma unroll
+  for (int i = 0; i < FM; i++)
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      sum[wave][0][16 * i + r][4 * (lane >> 4) + k] = ag[i][k];
+      sum[wave][1][16 * i + r][4 * (lane >> 4) + k] = au[i][k];
+    }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 256 * FM; e += 512) {
+    const int m = e / 16, c = e % 16;
+    if (m >= M || n0 + c >= F) continue;
+    float g = 0.0f, u = 0.0f, d;
+#pragma unroll
+    for (int w = 0; w < kW; w++) {
+      g += sum[w][0][m][c];
+      u += sum[w][1][m][c];
+    }
+    h[(int64_t)m * F + n0 + c] = from_f32<T>(act<ACT>(g, d) * u);
+  }
+}
+
+// dx and dW: plain products; a split of K leaves its sums in partial[split][matrix][M][N]
+struct PlainOut {
+  void *C[2];
+  int64_t ldc;
+  float *partial;
+};
+template <typename T, int BM, int BN, int WM, int WN, bool A_KO, bool B_KO, int PAIR>
+__global__ __launch_bounds__(64 * WM *WN) void product_kernel(const GemmArgs g, const PlainOut o) {
+  using G = Gemm<T, BM, BN, WM, WN, A_KO, B_KO, PAIR>;
+  DGS_GEMM_LDS(G)
+  const Where at = where_of(g.tiles_m, g.tiles_n);
+  const int z = PAIR == kTwo ? at.z % 2 : 0, split = PAIR == kTwo ? at.z / 2 : at.z;
+  const int m0 = at.m * BM, n0 = at.n * BN;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, wm = wave / WN, wn = wave % WN;
+  const int steps = (int)((g.K + G::TA::kK - 1) / G::TA::kK), all = PAIR == kSum ? 2 * steps : steps;
+  const int per = (all + g.splits - 1) / g.splits, s0 = split * per, s1 = s0 + per < all ? s0 + per : all;
+  f32x4 acc[G::FM][G::FN];
+  gemm_loop<G>(g, m0, n0, s0, s1, steps, z, A_KO, B_KO, sizeof(T), ldsA0, ldsB0, ldsA1, ldsB1, wm, wn, lane, acc);
+#pragma unroll
+  for (int i = 0; i < G::FM; i++) {
+    const int64_t m = m0 + wm * (BM / WM) + 16 * i + (lane & 15);
+    if (m >= g.M) continue;
+#pragma unroll
+    for (int j = 0; j < G::FN; j++) {
+      const int64_t n = n0 + G::c_col(wn, j) + 4 * (lane >> 4);
+      if (n >= g.N) continue;
+      if (o.partial) {
+        const int64_t mat = (int64_t)split * (PAIR == kTwo ? 2 : 1) + z;
+        store4<float>(o.partial + (mat * g.M + m) * g.N + n, acc[i][j], g.N - n, g.N % 4 == 0);
+      } else {
+        store4<T>((T *)o.C[z] + m * o.ldc + n, acc[i][j], g.N - n, o.ldc % 4 == 0);
+      }
+    }
+  }
+}
+static bool fits(int64_t M, int64_t N) {  // tiles of the smallest shape in a launch's x dimension
+  return ((M + 63) / 64) * ((N + 31) / 32) < INT32_MAX;
+}
+
+struct Layout {
+  bool pad;          // x and the weights are copied into padded rows
+  int64_t ldx, ldg;  // in elements: of x and the weights, and of dg and du
+  size_t x, wg, wu, dg, du, partial, total;
+};
+template <typename T>
+static Layout layout(int64_t rows, int64_t D, int64_t F, bool backward, int64_t ldx) {
+  Layout L;
+  size_t at = 0;
+  auto take = [&](size_t b) { const size_t o = at; at += round_up(b, 256); return o; };
+  constexpr int V = kVec<T>;
+  L.pad = D % V != 0;
+  L.ldx = L.pad ? (D + V - 1) / V * V : ldx;
+  L.ldg = (F + V - 1) / V * V;
+  L.x = take(L.pad ? (size_t)rows * L.ldx * sizeof(T) : 0);
+  L.wg = take(L.pad ? (size_t)F * L.ldx * sizeof(T) : 0);
+  L.wu = take(L.pad ? (size_t)F * L.ldx * sizeof(T) : 0);
+  L.dg = take(backward ? (size_t)rows * L.ldg * sizeof(T) : 0);
+  L.du = take(backward ? (size_t)rows * L.ldg * sizeof(T) : 0);
+  size_t part = 0;
+  if (backward) {
+    constexpr int kK = kStepBytes / (int)sizeof(T);
+    const TilePlan px = tile_plan(rows, D, 2 * ((F + kK - 1) / kK), 1, false, sizeof(T) == 2, true);
+    const TilePlan pw = tile_plan(F, D, (rows + kK - 1) / kK, 2, false, sizeof(T) == 2, true);
+    const size_t bx = px.splits > 1 ? (size_t)px.splits * rows * D * 4 : 0, bw = pw.splits > 1 ? (size_t)pw.splits * 2 * F * D * 4 : 0;
+    part = bx > bw ? bx : bw;
+  }
+  L.partial = take(part);
+  L.total = at;
+  return L;
+}
+
+template <typename T>
+struct Operands { const char *x, *wg, *wu; int64_t ldx, ldw; };  // strides in elements
+// x and the weights as the 16-byte loads want them
+template <typename T>
+static int operands(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, char *ws, const Layout &L, hipStream_t st,
+                    Operands<T> &o) {
+  if (!L.pad) {
+    if (!rows16(x, D, ldx, sizeof(T)) || !rows16(wg, D, ldw, sizeof(T)) || !rows16(wu, D, ldw, sizeof(T))) return DGS_EINVAL;
+    o = {(const char *)x, (const char *)wg, (const char *)wu, ldx, ldw};
+    return DGS_OK;
+  }
+  int rc = pad_rows<T>(rows, D, x, ldx, L.ldx, ws + L.x, st);
+  if (rc == DGS_OK) rc = pad_rows<T>(F, D, wg, ldw, L.ldx, ws + L.wg, st);
+  if (rc == DGS_OK) rc = pad_rows<T>(F, D, wu, ldw, L.ldx, ws + L.wu, st);
+  o = {ws + L.x, ws + L.wg, ws + L.wu, L.ldx, L.ldx};
+  return rc;
+}
+
+template <typename T, int ACT, bool BWD>
+static int launch_gated(int64_t rows, int64_t D, int64_t F, const Operands<T> &op, const GatedOut &out, hipStream_t st) {
+  constexpr int kK = kStepBytes / (int)sizeof(T);
+  const int64_t cols = BWD ? out.ldo : F;
+  const TilePlan p = tile_plan(rows, cols, (D + kK - 1) / kK, 1, true, sizeof(T) == 2, false);
+  GemmArgs g = {{op.x, nullptr}, {op.wg, op.wu}, op.ldx * (int64_t)sizeof(T), op.ldw * (int64_t)sizeof(T), rows, F, D, p.tiles_m, p.tiles_n, 1};
+  const dim3 grid((unsigned)(p.tiles_m * p.tiles_n));
+  if constexpr (sizeof(T) == 2) {
+    if (p.shape == kBig) {
+      hipLaunchKernelGGL((gated_kernel<T, 256, 256, 2, 4, ACT, BWD>), grid, dim3(512), 0, st, g, out);
+      return check_launch();
+    }
+  }
+  if (p.shape == kMid)
+    hipLaunchKernelGGL((gated_kernel<T, 128, 128, 2, 2, ACT, BWD>), grid, dim3(256), 0, st, g, out);
+  else
+    hipLaunchKernelGGL((gated_kernel<T, 64, 64, 2, 2, ACT, BWD>), grid, dim3(256), 0, st, g, out);
+  return check_launch();
+}
+template <typename T, bool A_KO, bool B_KO, int PAIR>
+static int launch_product(GemmArgs g, PlainOut o, const TilePlan &p, float *partial, hipStream_t st) {
+  constexpr int mats = PAIR == kTwo ? 2 : 1;
+  g.tiles_m = p.tiles_m;
+  g.tiles_n = p.tiles_n;
+  g.splits = p.splits;
+  o.partial = p.splits > 1 ? partial : nullptr;
+  const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)(p.splits * mats));
+  bool done = false;
+  if constexpr (sizeof(T) == 2) {
+    if (p.shape == kBig) {
+      hipLaunchKernelGGL((product_kernel<T, 256, 256, 2, 4, A_KO, B_KO, PAIR>), grid, dim3(512), 0, st, g, o);
+      done = true;
+    }
+  }
+  if (!done && p.shape == kMid)
+    hipLaunchKernelGGL((product_kernel<T, 128, 128, 2, 2, A_KO, B_KO, PAIR>), grid, dim3(256), 0, st, g, o);
+  else if (!done)
+    hipLaunchKernelGGL((product_kernel<T, 64, 64, 2, 2, A_KO, B_KO, PAIR>), grid, dim3(256), 0, st, g, o);
+  if (check_launch() != DGS_OK) return DGS_ELAUNCH;
+  if (p.splits > 1) {
+    const int64_t each = g.M * g.N, count = each * mats;
+    hipLaunchKernelGGL((join_splits_kernel<T>), dim3((unsigned)((count + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, count, p.splits, partial, (T *)o.C[0], (T *)o.C[1], each);
+    return check_launch();
+  }
+  return DGS_OK;
+}
+
+constexpr int64_t kFewRows = 64;
+
+template <typename T, int ACT>
+static int ffn_fwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, void *h, char *ws, hipStream_t st) {
+  const Layout L = layout<T>(rows, D, F, false, ldx);
+  Operands<T> op;
+  const int rc = operands<T>(rows, D, F, x, ldx, wg, wu, ldw, ws, L, st, op);
+  if (rc != DGS_OK) return rc;
+  if (rows <= kFewRows) {
+    const dim3 grid((unsigned)((F + 15) / 16));
+    const int64_t kb = (int64_t)(L.pad ? L.ldx : D) * (int64_t)sizeof(T), lx = op.ldx * (int64_t)sizeof(T), lw = op.ldw * (int64_t)sizeof(T);
+#define DGS_FEW(FM_) hipLaunchKernelGGL((gated_few_kernel<T, FM_, ACT>), grid, dim3(512), 0, st, op.x, lx, op.wg, op.wu, lw, (int)rows, F, kb, (T *)h)
+    if (rows <= 16) DGS_FEW(1);
+    else if (rows <= 32) DGS_FEW(2);
+    else DGS_FEW(4);
+#undef DGS_FEW
+    return check_launch();
+  }
+  const GatedOut out = {nullptr, h, nullptr, F, F};
+  return launch_gated<T, ACT, false>(rows, D, F, op, out, st);
+}
+
+template <typename T, int ACT>
+static int ffn_bwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, const void *dh, void *dx, void *dwg, void *dwu,
+                   char *ws, hipStream_t st) {
+  const Layout L = layout<T>(rows, D, F, true, ldx);
+  Operands<T> op;
+  int rc = operands<T>(rows, D, F, x, ldx, wg, wu, ldw, ws, L, st, op);
+  if (rc != DGS_OK) return rc;
+  constexpr int64_t size = sizeof(T);
+  constexpr int kK = kStepBytes / (int)sizeof(T);
+  char *dg = ws + L.dg, *du = ws + L.du;
+  const GatedOut out = {dh, dg, du, F, L.ldg};
+  rc = launch_gated<T, ACT, true>(rows, D, F, op, out, st);
+  float *partial = (float *)(ws + L.partial);
+  if (rc == DGS_OK && dx) {  // dx [rows, D] = dg Wg + du Wu: K = F, the weights K-outer
+    GemmArgs g = {{dg, du}, {op.wg, op.wu}, L.ldg * size, op.ldw * size, rows, D, F, 0, 0, 1};
+    PlainOut o = {{dx, nullptr}, D, nullptr};
+    rc = launch_product<T, false, true, kSum>(g, o, tile_plan(rows, D, 2 * ((F + kK - 1) / kK), 1, false, size == 2, true), partial, st);
+  }
+  if (rc == DGS_OK && dwg) {  // dWg, dWu [F, D] = dg^T x, du^T x: K = rows, both operands K-outer
+    GemmArgs g = {{dg, du}, {op.x, nullptr}, L.ldg * size, op.ldx * size, F, D, rows, 0, 0, 1};
+    PlainOut o = {{dwg, dwu}, D, nullptr};
+    rc = launch_product<T, true, true, kTwo>(g, o, tile_plan(F, D, (rows + kK - 1) / kK, 2, false, size == 2, true), partial, st);
+  }
+  return rc;
+}
+
+}  // namespace dgs
+
+using namespace dgs;
+
+static int ffn_sizes(int dtype, int activation, int64_t rows, int64_t D, int64_t F, int64_t ldx, int64_t ldw) {
+  if (!dtype_ok(dtype) || activation < DGS_ACT_SILU || activation > DGS_ACT_RELU || rows < 0 || D <= 0 || F <= 0 || ldx < 0 || ldw < 0) return DGS_EINVAL;
+  const int64_t size = (int64_t)dtype_bytes(dtype);
+  // offsets within a tile are 32 bits wide: 256 rows of any operand
+  const int64_t most = INT32_MAX / 256 / size - 64;
+  if (rows > INT32_MAX / 2 || D > most || F > most || ldx > most || ldw > most || !fits(rows, F) || !fits(rows, D) || !fits(F, D)) return DGS_ERANGE;
+  return DGS_OK;
+}
+
+extern "C" size_t dgs_gated_ffn_workspace_bytes(int dtype, int64_t rows, int64_t D, int64_t F, int backward) {
+  if (!dtype_ok(dtype) || rows <= 0 || D <= 0 || F <= 0) return 0;
+  return dtype == DGS_F32 ? layout<float>(rows, D, F, backward, D).total : layout<f16>(rows, D, F, backward, D).total;
+}
+
+#define DGS_ACTS(T, CALL)                                      \
+  switch (activation) {                                        \
+    case DGS_ACT_SILU: return CALL<T, DGS_ACT_SILU> ARGS;      \
+    case DGS_ACT_GELU: return CALL<T, DGS_ACT_GELU> ARGS;      \
+    default: return CALL<T, DGS_ACT_RELU> ARGS;                \
+  }
+
+extern "C" int dgs_gated_ffn(int dtype, int activation, int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *w_gate, const void *w_up, int64_t ldw,
+                             void *h, void *workspace, size_t workspace_bytes, dgsStream_t stream) {
+  const int rc = ffn_sizes(dtype, activation, rows, D, F, ldx, ldw);
+  if (rc != DGS_OK) return rc;
+  if (rows == 0) return DGS_OK;
+  if (!x || !w_gate || !w_up || !h || !aligned_to(h, 16)) return DGS_EINVAL;
+  const size_t need = dgs_gated_ffn_workspace_bytes(dtype, rows, D, F, 0);
+  if (need && (!workspace || workspace_bytes < need)) return DGS_EWORKSPACE;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char *ws = static_cast<char *>(workspace);
+#define ARGS (rows, D, F, x, ldx, w_gate, w_up, ldw, h, ws, st)
+  if (dtype == DGS_F32) DGS_ACTS(float, ffn_fwd)
+  if (dtype == DGS_F16) DGS_ACTS(f16, ffn_fwd)
+  DGS_ACTS(bf16, ffn_fwd)
+#undef ARGS
+}
+
+extern "C" int dgs_gated_ffn_bwd(int dtype, int activation, int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *w_gate, const void *w_up, int64_t ldw,
+                                 const void *dh, void *dx, void *dw_gate, void *dw_up, void *workspace, size_t workspace_bytes, dgsStream_t stream) {
+  const int rc = ffn_sizes(dtype, activation, rows, D, F, ldx, ldw);
+  if (rc != DGS_OK) return rc;
+  if (rows == 0 || !x || !w_gate || !w_up || !dh || !dw_gate != !dw_up || !aligned_to(dh, 16) || !aligned_to(dx, 16) || !aligned_to(dw_gate, 16) || !aligned_to(dw_up, 16))
+    return DGS_EINVAL;
+  const size_t need = dgs_gated_ffn_workspace_bytes(dtype, rows, D, F, 1);
+  if (!workspace || workspace_bytes < need) return DGS_EWORKSPACE;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char *ws = static_cast<char *>(workspace);
+#define ARGS (rows, D, F, x, ldx, w_gate, w_up, ldw, dh, dx, dw_gate, dw_up, ws, st)
+  if (dtype == DGS_F32) DGS_ACTS(float, ffn_bwd)
+  if (dtype == DGS_F16) DGS_ACTS(f16, ffn_bwd)
+  DGS_ACTS(bf16, ffn_bwd)
+#undef ARGS
+}

@@ -1,0 +1,353 @@
+// gemm_core.h -- tiled matrix product on the matrix cores of gfx950, the core of the gated feed-forward block and the 8-bit product.
+//
+//   C[m, n] = sum over k of A(m, k) B(n, k)
+//
+// An operand lies in memory either K-inner (row m holds its K values side by side) or K-outer (row k holds the M values side by side, as
+// in the gradients); neither is ever transposed in memory.  A workgroup of WM x WN waves makes a BM x BN tile of C, 128 bytes of K a step:
+//   * global -> LDS by the buffer unit (16 bytes a lane, no registers in between), two LDS buffers, the next step's loads in flight while
+//     this step's matrix instructions run.  Rows and K values behind the matrix read as zeros (their lanes ask for an offset behind the
+//     descriptor's range).
+//   * LDS -> registers: 16 bytes a lane = 16 rows x 64 bytes of K ("slice") for one 16 x 16 x (64 bytes) matrix step.  K-inner tiles are
+//     read with ds_read_b128, K-outer tiles with the transposing ds_read_b64_tr_b16 (16-bit types) or dword reads (32-bit).
+//   * The 16-byte pieces of an LDS row are permuted (XOR with some bits of the row), so that the rows that are read together lie in
+//     different banks; the loads fetch the pieces in that order, the LDS side of a load being a straight line by construction.
+//   * The operands enter the matrix instruction as (B, A): a lane then holds four neighbouring n of one row m, which leave in one store.
+// Sums are held in 32 bits throughout; K is walked in order, so a result depends on the tile shape and the number of splits alone, and
+// these on the sizes alone.
+#pragma once
+#include "dense_common.h"
+
+namespace dgs {
+
+struct fp8 { uint8_t v; };  // e4m3 (the OCP form: bias 7, no infinities)
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kStepBytes = 128;        // of K, a step
+constexpr uint32_t kNowhere = 0x80000000u;  // an offset behind every descriptor's range: reads as zero
+constexpr int kRange = 0x7ffffff0;     // the descriptors' range: offsets within a tile stay below it (checked by the dispatch)
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) char lds_char;
+
+// 16 bytes of K for each of 16 rows (per lane: one row, 16 bytes): one step of the matrix cores over 64 bytes of K
+union Slice {
+  dgs_u4 u;
+  bf16x8 b;
+  f16x8 h;
+  float f[4];
+  s16x4 s[2];
+};
+template <typename T> struct Mma;
+template <> struct Mma<bf16> {
+  static __device__ __forceinline__ void step(f32x4 &c, const Slice &b, const Slice &a) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.b, a.b, c, 0, 0, 0); }
+};
+template <> struct Mma<f16> {
+  static __device__ __forceinline__ void step(f32x4 &c, const Slice &b, const Slice &a) { c = __builtin_amdgcn_mfma_f32_16x16x32_f16(b.h, a.h, c, 0, 0, 0); }
+};
+template <> struct Mma<float> {  // lane group g holds k = 4 g .. 4 g + 3: the j-th of four instructions takes the j-th of them
+  static __device__ __forceinline__ void step(f32x4 &c, const Slice &b, const Slice &a) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(b.f[j], a.f[j], c, 0, 0, 0);
+  }
+};
+
+// ---- one operand's tile in LDS: R rows (of M or N) x 128 bytes of K, R * 128 bytes -------------------------------------------------
+template <typename T, int R, bool KO>
+struct Tile {
+  static constexpr int kBytes = R * kStepBytes;
+  static constexpr int kK = kStepBytes / (int)sizeof(T);       // K values a step
+  static constexpr int kCpr = KO ? R * (int)sizeof(T) / 16 : 8;  // 16-byte pieces of an LDS row (K-outer: a row is one k)
+
+  // which piece of the row the LDS place `slot` holds (and the other way round): rows that are read together go to different banks
+  static __device__ __forceinline__ int mix(int row, int slot) {
+    if constexpr (!KO) return slot ^ ((row >> 1) & 7);
+    else if constexpr (sizeof(T) == 2) return slot ^ (2 * (row & (kCpr / 2 - 1) & 7));
+    else return slot ^ (4 * ((row >> 2) & (kCpr / 4 - 1) & 3));
+  }
+  // byte offset of piece `id` (of R * 8, in LDS order) from the tile's corner; kNowhere if the row / column is behind the matrix.  `left`:
+  // rows of M (K-inner) or bytes of a row (K-outer) from the corner to the end of the matrix.
+  static __device__ __forceinline__ uint32_t offset(int id, int64_t ld, int64_t left, int &k) {
+    const int row = id / kCpr, piece = mix(row, id % kCpr);
+    if constexpr (!KO) {
+      k = piece * (16 / (int)sizeof(T));
+      return row < left ? (uint32_t)(row * ld + piece * 16) : kNowhere;
+    } else {
+      k = row;
+      return piece * 16 < left ? (uint32_t)(row * ld + piece * 16) : kNowhere;
+    }
+  }
+  // the slice of rows [16 i, 16 i + 16), 64 bytes kk of K
+  static __device__ __forceinline__ void read(const char *lds, int row0, int kk, int lane, Slice &s) {
+    if constexpr (!KO) {
+      const int row = row0 + (lane & 15), slot = mix(row, (lane >> 4) + 4 * kk);
+      s.u = *reinterpret_cast<const dgs_u4 *>(lds + row * kStepBytes + slot * 16);
+    } else if constexpr (sizeof(T) == 2) {
+      // each 16 lanes read 4 k x 16 m (8 bytes a lane) and get them transposed: a lane has the 4 k of its m
+      const int i = lane & 15;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int k = 32 * kk + 8 * (lane >> 4) + 4 * h + (i >> 2);
+        const int byte = row0 * 2 + (i & 3) * 8;
+        const char *p = lds + k * (kCpr * 16) + mix(k, byte / 16) * 16 + byte % 16;
+        s.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds_char *)p);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int k = 16 * kk + 4 * (lane >> 4) + j;
+        const int byte = (row0 + (lane & 15)) * 4;
+        s.f[j] = *reinterpret_cast<const float *>(lds + k * (kCpr * 16) + mix(k, byte / 16) * 16 + byte % 16);
+      }
+    }
+  }
+};
+
+// What a launch multiplies.  Leading dimensions in bytes.  `pair`: how the second pointers are used:
+//   kOne     C[0] = A[0] B[0]
+//   kDual    the tile's columns come in halves from B[0] and B[1] (BN / 2 columns each): C0 = A[0] B[0], C1 = A[0] B[1]
+//   kSum     C[0] = A[0] B[0] + A[1] B[1]   (one walk over K after the other)
+//   kTwo     C[0] = A[0] B[0], C[1] = A[1] B[0]  (workgroups for one, then for the other)
+enum Pair { kOne, kDual, kSum, kTwo };
+struct GemmArgs {
+  const char *A[2], *B[2];
+  int64_t lda, ldb;
+  int64_t M, N, K;  // N: of one matrix (kDual: columns of C0)
+  int tiles_m, tiles_n, splits;
+};
+
+// Which tile a workgroup makes.  Workgroups go round the 8 XCDs, each with an L2 of its own: XCD x takes the x-th eighth of the tiles, in
+// panels of kPanel tile rows, so that the tiles that run together on an XCD share their rows of A and columns of B there.
+constexpr int kXcds = 8, kPanel = 8;
+struct Where { int m, n, z; };
+__device__ __forceinline__ Where where_of(int tiles_m, int tiles_n) {
+  const int total = tiles_m * tiles_n;
+  int b = (int)blockIdx.x;
+  const int each = total / kXcds, rest = total % kXcds, x = b % kXcds;
+  b = b / kXcds + x * each + (x < rest ? x : rest);
+  const int panel = b / (kPanel * tiles_n), in = b % (kPanel * tiles_n);
+  const int rows = tiles_m - panel * kPanel < kPanel ? tiles_m - panel * kPanel : kPanel;
+  return {panel * kPanel + in % rows, in / rows, (int)blockIdx.y};
+}
+
+// The tile's sums: acc[i][j] = 16 x 16 at rows 16 i, columns col_of(j) of the wave's part; lane l register r holds m = l % 16, n = 4 (l / 16) + r.
+// STEP(i, j, part) is called for each 128 bytes of K where SCALED (8-bit types) instead of accumulating straight on.
+template <typename T, int BM, int BN, int WM, int WN, bool A_KO, bool B_KO, int PAIR>
+struct Gemm {
+  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  using TA = Tile<T, BM, A_KO>;
+  using TB = Tile<T, BN, B_KO>;
+  static constexpr int QA = BM * 8 / kThreads, QB = BN * 8 / kThreads;  // 16-byte loads of a thread a step
+  static constexpr int kCols = PAIR == kDual ? BN / 2 : BN;             // columns of C that a tile covers
+  static_assert(QA * kThreads == BM * 8 && QB * kThreads == BN * 8, "whole loads");
+  static_assert(PAIR != kDual || (!B_KO && QB % 2 == 0), "halves of the loads");
+
+  // column of the tile's B rows where the wave's j-th 16 columns begin, and the column of C
+  static __device__ __forceinline__ int b_row(int wn, int j) {
+    if constexpr (PAIR == kDual) return (j < FN / 2 ? 0 : BN / 2) + wn * (BN / 2 / WN) + 16 * (j % (FN / 2));
+    return wn * (BN / WN) + 16 * j;
+  }
+  static __device__ __forceinline__ int c_col(int wn, int j) {
+    if constexpr (PAIR == kDual) return wn * (BN / 2 / WN) + 16 * (j % (FN / 2));
+    return wn * (BN / WN) + 16 * j;
+  }
+
+  struct Load {  // one thread's share of a step's loads
+    uint32_t a[QA], b[QB];
+    int ka[QA], kb[QB];
+  };
+  static __device__ __forceinline__ void plan(Load &l, const GemmArgs &g, int m0, int n0) {
+#pragma unroll
+    for (int q = 0; q < QA; q++)
+      l.a[q] = TA::offset(q * kThreads + (int)threadIdx.x, g.lda, A_KO ? ((g.M - m0) * (int64_t)sizeof(T) + 15) / 16 * 16 : g.M - m0, l.ka[q]);
+#pragma unroll
+    for (int q = 0; q < QB; q++) {
+      if constexpr (PAIR == kDual) {  // both halves alike
+        l.b[q] = TB::offset((q % (QB / 2)) * kThreads + (int)threadIdx.x, g.ldb, g.N - n0, l.kb[q]);
+      } else {
+        l.b[q] = TB::offset(q * kThreads + (int)threadIdx.x, g.ldb, B_KO ? ((g.N - n0) * (int64_t)sizeof(T) + 15) / 16 * 16 : g.N - n0, l.kb[q]);
+      }
+    }
+  }
+  // The loads of step s (of `steps` a walk over K; kSum: 2 * steps in all) into one LDS buffer
+  static __device__ __forceinline__ void load(const Load &l, const GemmArgs &g, int s, int steps, int z, int64_t a_at, int64_t b_at, char *la, char *lb) {
+    const int seg = PAIR == kSum ? (s >= steps ? 1 : 0) : 0;
+    const int st = s - seg * steps;
+    const int left = (int)(g.K - (int64_t)st * TA::kK < TA::kK ? g.K - (int64_t)st * TA::kK : TA::kK);  // K values of this step
+    const char *pa = g.A[PAIR == kTwo ? z : seg] + a_at + (A_KO ? (int64_t)st * TA::kK * g.lda : (int64_t)st * kStepBytes);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    {
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pa), 0, kRange, 0x00027000);
+#pragma unroll
+      for (int q = 0; q < QA; q++)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds_char *)(la + (q * kWaves + wave) * 1024), 16, l.ka[q] < left ? (int)l.a[q] : (int)kNowhere, 0, 0, 0);
+    }
+#pragma unroll
+    for (int half = 0; half < (PAIR == kDual ? 2 : 1); half++) {
+      const char *pb = g.B[PAIR == kDual ? half : seg] + b_at + (B_KO ? (int64_t)st * TB::kK * g.ldb : (int64_t)st * kStepBytes);
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pb), 0, kRange, 0x00027000);
+      constexpr int per = PAIR == kDual ? QB / 2 : QB;
+#pragma unroll
+      for (int q = 0; q < per; q++)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds_char *)(lb + ((half * per + q) * kWaves + wave) * 1024), 16, l.kb[q] < left ? (int)l.b[q] : (int)kNowhere, 0, 0, 0);
+    }
+  }
+  static __device__ __forceinline__ void compute(const char *la, const char *lb, int wm, int wn, int lane, f32x4 (&acc)[FM][FN]) {
+#pragma unroll
+    for (int kk = 0; kk < 2; kk++) {
+      __builtin_amdgcn_sched_barrier(0);  // (one half's operands in registers at a time)
+      Slice a[FM], b[FN];
+#pragma unroll
+      for (int j = 0; j < FN; j++) TB::read(lb, b_row(wn, j), kk, lane, b[j]);
+#pragma unroll
+      for (int i = 0; i < FM; i++) TA::read(la, wm * (BM / WM) + 16 * i, kk, lane, a[i]);
+#pragma unroll
+      for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) Mma<T>::step(acc[i][j], b[j], a[i]);
+    }
+  }
+};
+
+// This wave's loads have landed in LDS and its LDS reads are done; then the workgroup's.  (Said outright: a barrier alone need not wait for
+// loads that go to LDS.)
+__device__ __forceinline__ void loads_done() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// The main loop, 16- and 32-bit types: steps [s0, s1) into acc.  The four LDS buffers are separate arrays, so that the compiler sees that
+// a step's reads and the next step's loads do not meet and does not wait for the loads in between.
+#define DGS_GEMM_LDS(G)                                              \
+  __shared__ __align__(16) char ldsA0[G::TA::kBytes], ldsB0[G::TB::kBytes]; \
+  __shared__ __align__(16) char ldsA1[G::TA::kBytes], ldsB1[G::TB::kBytes];
+
+template <typename G>
+__device__ __forceinline__ void gemm_loop(const GemmArgs &g, int m0, int n0, int s0, int s1, int steps, int z, bool a_ko, bool b_ko, size_t elem, char *ldsA0,
+                                          char *ldsB0, char *ldsA1, char *ldsB1, int wm, int wn, int lane, f32x4 (&acc)[G::FM][G::FN]) {
+#pragma unroll
+  for (int i = 0; i < G::FM; i++)
+#pragma unroll
+    for (int j = 0; j < G::FN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (s0 >= s1) return;
+  typename G::Load l;
+  G::plan(l, g, m0, n0);
+  const int64_t a_at = a_ko ? (int64_t)m0 * (int64_t)elem : (int64_t)m0 * g.lda, b_at = b_ko ? (int64_t)n0 * (int64_t)elem : (int64_t)n0 * g.ldb;
+  G::load(l, g, s0, steps, z, a_at, b_at, ldsA0, ldsB0);
+  loads_done();
+  int s = s0;
+  for (; s + 1 < s1; s += 2) {  // (no way out in the middle: the sums would be moved between registers there)
+    G::load(l, g, s + 1, steps, z, a_at, b_at, ldsA1, ldsB1);
+    G::compute(ldsA0, ldsB0, wm, wn, lane, acc);
+    loads_done();
+    if (s + 2 < s1) G::load(l, g, s + 2, steps, z, a_at, b_at, ldsA0, ldsB0);
+    G::compute(ldsA1, ldsB1, wm, wn, lane, acc);
+    loads_done();
+  }
+  if (s < s1) G::compute(ldsA0, ldsB0, wm, wn, lane, acc);
+}
+
+// four neighbouring columns of a row; `vec`: the row's stride and base allow one store
+template <typename T>
+__device__ __forceinline__ void store4(T *p, const f32x4 &v, int64_t left, bool vec) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<f32x4 *>(p) = v;
+    } else {
+      union { dgs_u2 u; T t[4]; } x;
+#pragma unroll
+      for (int k = 0; k < 4; k++) x.t[k] = from_f32<T>(v[k]);
+      *reinterpret_cast<dgs_u2 *>(p) = x.u;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (k < left) p[k] = from_f32<T>(v[k]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T *p, int64_t left, bool vec) {
+  f32x4 v;
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      v = *reinterpret_cast<const f32x4 *>(p);
+    } else {
+      union { dgs_u2 u; T t[4]; } x;
+      x.u = *reinterpret_cast<const dgs_u2 *>(p);
+#pragma unroll
+      for (int k = 0; k < 4; k++) v[k] = to_f32(x.t[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = k < left ? to_f32(p[k]) : 0.0f;
+  }
+  return v;
+}
+
+// Rows of another stride than the 16-byte loads take: copied once, padded with zeros to a multiple of 16 bytes.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void pad_rows_kernel(int64_t rows, int64_t cols, const T *__restrict__ src, int64_t ld, int64_t ldo, T *__restrict__ dst) {
+  const int64_t t = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int64_t per = ldo * (int64_t)sizeof(T) / 16, row = t / per, c = t % per * (16 / (int64_t)sizeof(T));
+  if (row >= rows) return;
+  union { dgs_u4 u; T t[16 / sizeof(T)]; } x;
+  x.u = dgs_u4{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int k = 0; k < 16 / (int)sizeof(T); k++)
+    if (c + k < cols) x.t[k] = src[row * ld + c + k];
+  *reinterpret_cast<dgs_u4 *>(dst + row * ldo + c) = x.u;
+}
+template <typename T>
+static int pad_rows(int64_t rows, int64_t cols, const void *src, int64_t ld, int64_t ldo, void *dst, hipStream_t st) {
+  const int64_t n = rows * (ldo * (int64_t)sizeof(T) / 16), blocks = (n + kBlock - 1) / kBlock;
+  if (blocks > INT32_MAX) return DGS_ERANGE;
+  hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)blocks), dim3(kBlock), 0, st, rows, cols, (const T *)src, ld, ldo, (T *)dst);
+  return check_launch();
+}
+inline bool rows16(const void *p, int64_t cols, int64_t ld, size_t size) {
+  return aligned_to(p, 16) && (cols * (int64_t)size) % 16 == 0 && (ld * (int64_t)size) % 16 == 0;
+}
+
+// C[e] = the splits' sums in their order
+template <typename T>
+__global__ __launch_bounds__(kBlock) void join_splits_kernel(int64_t count, int splits, const float *__restrict__ partial, T *__restrict__ c0, T *__restrict__ c1, int64_t each) {
+  const int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (e >= count) return;
+  float s = 0.0f;
+#pragma unroll 4
+  for (int z = 0; z < splits; z++) s += partial[z * count + e];
+  if (e < each) c0[e] = from_f32<T>(s); else c1[e - each] = from_f32<T>(s);
+}
+
+// ---- which tile, how many splits ------------------------------------------------------------------------------------------
+// kBig: 256 x 256, 8 waves, a workgroup a CU; kMid: 128 x 128, 4 waves, 2 a CU; kSmall: 64 x 64, 4 waves.  A larger tile reads less from L2
+// and LDS for a product, but there have to be enough of them: the largest whose tiles (times splits of K, where the caller can split)
+// fill three quarters of the CUs.
+enum Shape { kBig, kMid, kSmall };
+struct TilePlan { Shape shape; int tiles_m, tiles_n, splits; };
+static TilePlan tile_plan(int64_t M, int64_t N, int64_t steps, int mats, bool dual, bool big, bool split) {
+  TilePlan p = {kSmall, 0, 0, 1};
+  const int sizes[] = {256, 128, 64};
+  const int64_t cus = cu_count(), want = cus * 3 / 4;
+  for (int s = big ? kBig : kMid; s <= kSmall; s++) {
+    const int64_t tm = (M + sizes[s] - 1) / sizes[s], cols = dual ? sizes[s] / 2 : sizes[s], tn = (N + cols - 1) / cols, tiles = tm * tn * mats;
+    p.shape = (Shape)s;
+    p.tiles_m = (int)tm;
+    p.tiles_n = (int)tn;
+    p.splits = 1;
+    if (tiles >= want) break;
+    if (split) {
+      const int64_t fill = (2 * cus + tiles - 1) / tiles, most = steps / (s == kSmall ? 4 : 16);
+      p.splits = (int)(fill < most ? fill : most < 1 ? 1 : most);
+      if (tiles * p.splits >= want) break;
+    }
+  }
+  return p;
+}
+
+}  // namespace dgs

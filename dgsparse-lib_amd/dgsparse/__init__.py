@@ -6,6 +6,7 @@ gfx950 HIP kernels reached through the C ABI of ``libdgsparse_hip.so`` (include/
 from . import _C  # noqa: F401  (reference: pybind module with cuda_version())
 from . import _capi  # noqa: F401  (raises ImportError if libdgsparse_hip.so is missing)
 from . import _ops  # noqa: F401  (registers torch.ops.dgsparse_spmm.*)
+from .dense import add_rms_norm, add_rms_norm_fp8, embedding, gated_ffn, matmul_fp8, quantize_fp8, rms_norm
 from .ftransform import csr2csc
 from .sddmm import sddmm
 from .spmm import spmm_max, spmm_mean, spmm_min, spmm_sum
@@ -25,4 +26,5 @@ ALG_NO_HUB_COLS = _capi.ALG_NO_HUB_COLS    # from what the Storage knows: Storag
 
 cuda_version = _C.cuda_version()  # -1 on ROCm: the reference's CUDA-major check is skipped (__init__.py:29)
 
-__all__ = ['spmm_sum', 'spmm_max', 'spmm_min', 'spmm_mean', 'sddmm', 'Storage', 'SparseTensor', 'csr2csc']
+__all__ = ['spmm_sum', 'spmm_max', 'spmm_min', 'spmm_mean', 'sddmm', 'Storage', 'SparseTensor', 'csr2csc',
+           'embedding', 'rms_norm', 'add_rms_norm', 'add_rms_norm_fp8', 'gated_ffn', 'quantize_fp8', 'matmul_fp8']

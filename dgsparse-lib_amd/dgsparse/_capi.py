@@ -153,7 +153,11 @@ EXPORTS = ['dgs_version', 'dgs_arch', 'dgs_strerror', 'dgs_reload_tuning', 'dgs_
            'dgs_csr2csc_i32', 'dgs_gather_rows_f32', 'dgs_scatter_add_rows_f32', 'dgs_relabel_i32', 'dgs_nonfinite_flag_f32', 'dgs_spmm_min_merge_f32', 'dgs_sddmm_coo_f32', 'dgs_gspmm_csr_workspace_bytes', 'dgs_gspmm_csr_f32', 'gespmmCsrSpMM',
            'spmm_cuda', 'spmm_cuda_no_edge_value', 'sddmm_cuda_csr', 'sddmm_cuda_coo', 'gespmmAlgSel',
            'csrspmm_parreduce_rowbalance', 'csrspmm_parreduce_nnzbalance', 'csrspmm_seqreduce_rowbalance',
-           'csrspmm_seqreduce_nnzbalance', 'csrspmm_rowcaching_rowbalance', 'csrspmm_rowcaching_nnzbalance']
+           'csrspmm_seqreduce_nnzbalance', 'csrspmm_rowcaching_rowbalance', 'csrspmm_rowcaching_nnzbalance',
+           # dense operators: bound by csrc/torch_dense.cpp (dgsparse/dense.py), not through ctypes
+           'dgs_embedding', 'dgs_embedding_bwd_workspace_bytes', 'dgs_embedding_bwd', 'dgs_rms_norm', 'dgs_rms_norm_bwd_workspace_bytes',
+           'dgs_rms_norm_bwd', 'dgs_gated_ffn_workspace_bytes', 'dgs_gated_ffn', 'dgs_gated_ffn_bwd', 'dgs_quantize_fp8',
+           'dgs_matmul_fp8_workspace_bytes', 'dgs_matmul_fp8']
 
 
 # ---- DGS_CANARY=1 (debug): every output and workspace this module allocates sits between two 4 KiB guard bands of a

@@ -425,6 +425,64 @@ int dgs_spmm_min_merge_f32(int64_t R, int64_t N, const int32_t *rowmap, const in
                            const int32_t *nonfinite, const int32_t *rowptr, const int32_t *col, const float *val,
                            const float *B, dgsStream_t stream);
 
+/* ---- dense operators around the sparse products (no counterpart in the reference, whose layers call torch for them) ----------------
+ *
+ * Element type of a call's tensors.  Sums, row statistics and running values are held in 32 bits whatever the type; a result is rounded
+ * to the type once, when it is stored.  Rows are contiguous (unit stride); `ld*` is the distance between rows in elements.  None of these
+ * entries allocates, synchronises or keeps state; they may be recorded into a graph (no memset nodes).  All of them return DGS_EINVAL
+ * for a null required pointer, a negative size or an unknown type, DGS_ERANGE for sizes beyond the indexing, DGS_EWORKSPACE for a
+ * workspace that is too small. */
+enum { DGS_F32 = 0, DGS_F16 = 1, DGS_BF16 = 2 };
+
+/* Embedding lookup: out[p, :] = scale * table[ids[p], :].  ids[n] of id_bytes = 4 | 8; table [V, D]; out [n, D] contiguous.  A negative id
+ * stands for "no token": its row is 0.  An id >= V is a mistake: nothing is read for it and its row is NaN. */
+int dgs_embedding(int dtype, int id_bytes, int64_t n, int64_t V, int64_t D, const void *ids, const void *table, int64_t ld_table,
+                  float scale, void *out, dgsStream_t stream);
+/* Its gradient: dtable[v, :] = scale * sum over p with ids[p] == v, in the order of p, of dout[p, :]; every row of dtable [V, D] is written.
+ * Ids that are negative, >= V or equal to padding_idx (< 0: none) add to no row.  Deterministic: positions are sorted by id, no atomics
+ * on values.  dout [n, D]; workspace dgs_embedding_bwd_workspace_bytes(), 256-byte aligned. */
+size_t dgs_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
+int dgs_embedding_bwd(int dtype, int id_bytes, int64_t n, int64_t V, int64_t D, const void *ids, int64_t padding_idx, const void *dout,
+                      int64_t ld_dout, float scale, void *dtable, void *workspace, size_t workspace_bytes, dgsStream_t stream);
+
+/* Root-mean-square norm over rows of D, with the residual's addition in front of it:
+ *   s = x + residual (rounded to the type: what the next layer adds to, and what the norm is taken of);  y = s / sqrt(mean(s^2) + eps) * w
+ * residual and s both null: y = norm(x).  Output either y [rows, D], or (y null) q [rows, D] in e4m3 with scales [rows, ceil(D / 128)]:
+ * scale = max|y| of 128 columns / 448 (at least 2^-96 / 448), q = y / scale; a NaN among the 128 makes the scale NaN.  x, residual with row
+ * distances ldx, ldr; everything else contiguous. */
+int dgs_rms_norm(int dtype, int64_t rows, int64_t D, const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *weight,
+                 float eps, void *y, void *s, uint8_t *q, float *scales, dgsStream_t stream);
+/* Its backward pass: dx [rows, D] = r w dy - s r^3 mean(s w dy) + ds (the gradient of x and of residual alike; ds may be null),
+ * dweight [D] = sum over rows of dy s r (may be null).  All contiguous. */
+size_t dgs_rms_norm_bwd_workspace_bytes(int dtype, int64_t rows, int64_t D);
+int dgs_rms_norm_bwd(int dtype, int64_t rows, int64_t D, const void *s, const void *weight, float eps, const void *dy, const void *ds,
+                     void *dx, void *dweight, void *workspace, size_t workspace_bytes, dgsStream_t stream);
+
+/* Gated feed-forward product: h [rows, F] = act(x Wg^T) * (x Wu^T);  x [rows, D] with row distance ldx, Wg and Wu [F, D] with row distance
+ * ldw, h contiguous and 16-byte aligned.  Where D is a multiple of 16 bytes, x, Wg and Wu have to lie at multiples of 16 bytes with row
+ * distances that are such too (else DGS_EINVAL); any other D is taken through padded copies in the workspace. */
+enum { DGS_ACT_SILU = 0, DGS_ACT_GELU = 1, DGS_ACT_RELU = 2 }; /* gelu: with the normal distribution (erf), not its tanh form */
+size_t dgs_gated_ffn_workspace_bytes(int dtype, int64_t rows, int64_t D, int64_t F, int backward);
+int dgs_gated_ffn(int dtype, int activation, int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *w_gate,
+                  const void *w_up, int64_t ldw, void *h, void *workspace, size_t workspace_bytes, dgsStream_t stream);
+/* Its backward pass, from dh [rows, F]: with g, u the two products, dg = dh u act'(g) and du = dh act(g) (rounded to the type: operands of
+ * the matrix cores), dx [rows, D] = dg Wg + du Wu (may be null), dWg = dg^T x and dWu = du^T x [F, D] (both or neither may be null).
+ * rows > 0; dh and the outputs contiguous, 16-byte aligned. */
+int dgs_gated_ffn_bwd(int dtype, int activation, int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *w_gate,
+                      const void *w_up, int64_t ldw, const void *dh, void *dx, void *dw_gate, void *dw_up, void *workspace,
+                      size_t workspace_bytes, dgsStream_t stream);
+
+/* x [rows, cols] in 8-bit floating point (e4m3): q [rows, cols] contiguous, scales [ceil(rows / block_rows), ceil(cols / 128)], one for each
+ * block_rows (1 or 128) x 128 values: max|x| / 448 (at least 2^-96 / 448; NaN if one of the values is), q = x / scale. */
+int dgs_quantize_fp8(int dtype, int64_t rows, int64_t cols, const void *x, int64_t ldx, int block_rows, uint8_t *q, float *scales,
+                     dgsStream_t stream);
+/* out [M, N] = A B^T of e4m3 operands: a [M, K] (row distance lda) with a_scale [M, ceil(K / 128)], b [N, K] (ldb) with b_scale
+ * [ceil(N / 128), ceil(K / 128)], all scales contiguous; out contiguous, 16-byte aligned, rounded once to out_dtype.  Where K is a multiple of
+ * 16, a and b have to lie at multiples of 16 bytes, their row distances too; any other K is taken through padded copies. */
+size_t dgs_matmul_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int dgs_matmul_fp8(int out_dtype, int64_t M, int64_t N, int64_t K, const uint8_t *a, int64_t lda, const float *a_scale, const uint8_t *b,
+                   int64_t ldb, const float *b_scale, void *out, void *workspace, size_t workspace_bytes, dgsStream_t stream);
+
 /* ---- GE-SpMM / SDDMM compatibility entry points (same names and argument order as the reference's
  *      standalone C libraries; default stream, void return) ------------------------------------- */
 
