@@ -62,18 +62,21 @@ __global__ __launch_bounds__(64 * WM *WN) void fp8_kernel(const GemmArgs g, cons
     for (int j = 0; j < G::FN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const int64_t nlast = (g.N - 1) / 128, nb = (n0 + wn * (BN / WN)) / 128;
   const float *sb = sc.b + (nb < nlast ? nb : nlast) * sc.blocks;
-  const float *sa[G::FM];
-  float f[G::FM], next[G::FM];
+  // the scales of a by a descriptor that ends with the matrix (rows behind it: 0), one offset for all 16-row parts
+  const int64_t scale_bytes = (g.M - m0) * sc.blocks * 4;
+  const auto sa = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(sc.a + m0 * sc.blocks), 0, scale_bytes < kRange ? (int)scale_bytes : kRange, 0x00027000);
+  const int sa_at = (wm * (BM / WM) + (lane & 15)) * (int)sc.blocks * 4;
+  float f[G::FM], raw[G::FM], raw_b = 0.0f;
+  auto fetch_scales = [&](int s) {  // (in front of the step's other loads: loads come back in order)
+    raw_b = sb[s];
 #pragma unroll
-  for (int i = 0; i < G::FM; i++) {
-    const int64_t m = m0 + wm * (BM / WM) + 16 * i + (lane & 15);
-    sa[i] = sc.a + (m < g.M ? m : g.M - 1) * sc.blocks;
-  }
-  auto scale = [&](int s, float (&to)[G::FM]) {
-#pragma unroll
-    for (int i = 0; i < G::FM; i++) to[i] = sa[i][s] * sb[s];
+    for (int i = 0; i < G::FM; i++) raw[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sa, sa_at + (16 * i * (int)sc.blocks + s) * 4, 0, 0));
   };
-  auto compute = [&](const char *la, const char *lb, const float (&f)[G::FM]) {
+  auto take_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < G::FM; i++) f[i] = raw[i] * raw_b;
+  };
+  auto compute = [&](const char *la, const char *lb) {
     Slice8 b[G::FN];
 #pragma unroll
     for (int j = 0; j < G::FN; j++)
@@ -102,30 +105,33 @@ __global__ __launch_bounds__(64 * WM *WN) void fp8_kernel(const GemmArgs g, cons
         const f32x4 part = block_product<T>(b[j], a[i & 1]);
 #pragma unroll
         for (int k = 0; k < 4; k++) acc[i][j][k] = __builtin_fmaf(part[k], f[i], acc[i][j][k]);
+        asm volatile("" : "+v"(acc[i][j]));  // (here, not behind all the products: their sums would fill the registers)
       }
     }
   };
   if (s0 < s1) {
     typename G::Load l;
     G::plan(l, g, m0, n0);
-    const int64_t a_at = (int64_t)m0 * g.lda, b_at = (int64_t)n0 * g.ldb;
-    G::load(l, g, s0, steps, 0, a_at, b_at, ldsA0, ldsB0);
-    scale(s0, f);
+    fetch_scales(s0);
+    G::load(l, g, m0, n0, s0, steps, 0, ldsA0, ldsB0);
     loads_done();
     int s = s0;
     for (; s + 1 < s1; s += 2) {
-      G::load(l, g, s + 1, steps, 0, a_at, b_at, ldsA1, ldsB1);
-      scale(s + 1, next);
-      compute(ldsA0, ldsB0, f);
+      take_scales();
+      fetch_scales(s + 1);
+      G::load(l, g, m0, n0, s + 1, steps, 0, ldsA1, ldsB1);
+      compute(ldsA0, ldsB0);
       loads_done();
+      take_scales();
       if (s + 2 < s1) {
-        G::load(l, g, s + 2, steps, 0, a_at, b_at, ldsA0, ldsB0);
-        scale(s + 2, f);
+        fetch_scales(s + 2);
+        G::load(l, g, m0, n0, s + 2, steps, 0, ldsA0, ldsB0);
       }
-      compute(ldsA1, ldsB1, next);
+      compute(ldsA1, ldsB1);
       loads_done();
     }
-    if (s < s1) compute(ldsA0, ldsB0, f);
+    take_scales();
+    if (s < s1) compute(ldsA0, ldsB0);
   }
 #pragma unroll
   for (int i = 0; i < G::FM; i++) {

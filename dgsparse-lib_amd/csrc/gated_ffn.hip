@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * WM *WN) void gated_kernel(const GemmArgs g, co
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, wm = wave / WN, wn = wave % WN;
   const int steps = (int)((g.K + G::TA::kK - 1) / G::TA::kK);
   f32x4 acc[G::FM][G::FN];
-  gemm_loop<G>(g, m0, n0, 0, steps, steps, 0, false, false, sizeof(T), ldsA0, ldsB0, ldsA1, ldsB1, wm, wn, lane, acc);
+  gemm_loop<G>(g, m0, n0, 0, steps, steps, 0, ldsA0, ldsB0, ldsA1, ldsB1, wm, wn, lane, acc);
   const bool vec = o.ldo % 4 == 0;
   const int64_t end = BWD ? o.ldo : o.F;
 #pragma unroll
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(64 * WM *WN) void product_kernel(const GemmArgs g, 
   const int steps = (int)((g.K + G::TA::kK - 1) / G::TA::kK), all = PAIR == kSum ? 2 * steps : steps;
   const int per = (all + g.splits - 1) / g.splits, s0 = split * per, s1 = s0 + per < all ? s0 + per : all;
   f32x4 acc[G::FM][G::FN];
-  gemm_loop<G>(g, m0, n0, s0, s1, steps, z, A_KO, B_KO, sizeof(T), ldsA0, ldsB0, ldsA1, ldsB1, wm, wn, lane, acc);
+  gemm_loop<G>(g, m0, n0, s0, s1, steps, z, ldsA0, ldsB0, ldsA1, ldsB1, wm, wn, lane, acc);
 #pragma unroll
   for (int i = 0; i < G::FM; i++) {
     const int64_t m = m0 + wm * (BM / WM) + 16 * i + (lane & 15);

@@ -28,7 +28,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kStepBytes = 128;        // of K, a step
-constexpr uint32_t kNowhere = 0x80000000u;  // an offset behind every descriptor's range: reads as zero
+constexpr uint32_t kNowhere = 0x80000000u;  // an offset behind every descriptor's range: reads as zero (and so does anything up to 2^31 behind it)
 constexpr int kRange = 0x7ffffff0;     // the descriptors' range: offsets within a tile stay below it (checked by the dispatch)
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -66,20 +66,22 @@ struct Tile {
   // which piece of the row the LDS place `slot` holds (and the other way round): rows that are read together go to different banks
   static __device__ __forceinline__ int mix(int row, int slot) {
     if constexpr (!KO) return slot ^ ((row >> 1) & 7);
-    else if constexpr (sizeof(T) == 2) return slot ^ (2 * (row & (kCpr / 2 - 1) & 7));
+    else if constexpr (sizeof(T) == 2) return slot ^ (2 * (((row & 3) + ((row >> 1) & 4)) & (kCpr / 2 - 1)));  // (4 rows and every second 8 rows are read together)
     else return slot ^ (4 * ((row >> 2) & (kCpr / 4 - 1) & 3));
   }
-  // byte offset of piece `id` (of R * 8, in LDS order) from the tile's corner; kNowhere if the row / column is behind the matrix.  `left`:
-  // rows of M (K-inner) or bytes of a row (K-outer) from the corner to the end of the matrix.
+  // A thread loads pieces id, id + THREADS, ... (of R * 8, in LDS order): kRowsPerLoad rows apart, at the same place of the row where the
+  // permutation does not change over that distance (kSame).
+  // offset(): of piece `id` from the tile's corner; K-outer: kNowhere where the piece lies behind the row's `left` bytes (rows behind the
+  // matrix are behind the descriptor's range for either kind).  k: its first K value in the step (K-inner).
   static __device__ __forceinline__ uint32_t offset(int id, int64_t ld, int64_t left, int &k) {
     const int row = id / kCpr, piece = mix(row, id % kCpr);
-    if constexpr (!KO) {
-      k = piece * (16 / (int)sizeof(T));
-      return row < left ? (uint32_t)(row * ld + piece * 16) : kNowhere;
-    } else {
-      k = row;
-      return piece * 16 < left ? (uint32_t)(row * ld + piece * 16) : kNowhere;
-    }
+    k = piece * (16 / (int)sizeof(T));
+    return !KO || piece * 16 < left ? (uint32_t)(row * (int)ld + piece * 16) : kNowhere;
+  }
+  template <int THREADS>
+  static constexpr bool same() {
+    constexpr int rows = THREADS / kCpr;  // a load further
+    return !KO ? rows % 16 == 0 : sizeof(T) == 2 ? rows % 16 == 0 : rows % 16 == 0;
   }
   // the slice of rows [16 i, 16 i + 16), 64 bytes kk of K
   static __device__ __forceinline__ void read(const char *lds, int row0, int kk, int lane, Slice &s) {
@@ -157,44 +159,62 @@ struct Gemm {
     return wn * (BN / WN) + 16 * j;
   }
 
-  struct Load {  // one thread's share of a step's loads
-    uint32_t a[QA], b[QB];
-    int ka[QA], kb[QB];
+  // One thread's share of a step's loads: the offset of the first, and of the others where they do not follow from it by the rows' distance.
+  static constexpr bool kSameA = TA::template same<kThreads>(), kSameB = TB::template same<kThreads>();
+  static constexpr int PB = PAIR == kDual ? QB / 2 : QB;  // loads of one B (kDual: both alike)
+  struct Load {
+    uint32_t a[kSameA ? 1 : QA], b[kSameB ? 1 : PB];
+    int ka, kb;
+    int da, db;  // kSame: bytes from one load's row to the next one's (the same in every lane)
   };
   static __device__ __forceinline__ void plan(Load &l, const GemmArgs &g, int m0, int n0) {
+    const int64_t left_a = ((g.M - m0) * (int64_t)sizeof(T) + 15) / 16 * 16, left_b = ((g.N - n0) * (int64_t)sizeof(T) + 15) / 16 * 16;
+    int k;
 #pragma unroll
-    for (int q = 0; q < QA; q++)
-      l.a[q] = TA::offset(q * kThreads + (int)threadIdx.x, g.lda, A_KO ? ((g.M - m0) * (int64_t)sizeof(T) + 15) / 16 * 16 : g.M - m0, l.ka[q]);
-#pragma unroll
-    for (int q = 0; q < QB; q++) {
-      if constexpr (PAIR == kDual) {  // both halves alike
-        l.b[q] = TB::offset((q % (QB / 2)) * kThreads + (int)threadIdx.x, g.ldb, g.N - n0, l.kb[q]);
-      } else {
-        l.b[q] = TB::offset(q * kThreads + (int)threadIdx.x, g.ldb, B_KO ? ((g.N - n0) * (int64_t)sizeof(T) + 15) / 16 * 16 : g.N - n0, l.kb[q]);
-      }
+    for (int q = 0; q < (kSameA ? 1 : QA); q++) {
+      l.a[q] = TA::offset(q * kThreads + (int)threadIdx.x, g.lda, left_a, k);
+      if (q == 0) l.ka = k;
     }
+#pragma unroll
+    for (int q = 0; q < (kSameB ? 1 : PB); q++) {
+      l.b[q] = TB::offset(q * kThreads + (int)threadIdx.x, g.ldb, left_b, k);
+      if (q == 0) l.kb = k;
+    }
+    l.da = kThreads / TA::kCpr * (int)g.lda;
+    l.db = kThreads / TB::kCpr * (int)g.ldb;
+  }
+  // bytes from a tile's corner to the matrix's last row's end, as a descriptor's range
+  static __device__ __forceinline__ int range(int64_t rows, int64_t ld) {
+    const int64_t b = rows * ld;
+    return b < kRange ? (int)b : kRange;
   }
   // The loads of step s (of `steps` a walk over K; kSum: 2 * steps in all) into one LDS buffer
-  static __device__ __forceinline__ void load(const Load &l, const GemmArgs &g, int s, int steps, int z, int64_t a_at, int64_t b_at, char *la, char *lb) {
+  static __device__ __forceinline__ void load(const Load &l, const GemmArgs &g, int m0, int n0, int s, int steps, int z, char *la, char *lb) {
     const int seg = PAIR == kSum ? (s >= steps ? 1 : 0) : 0;
     const int st = s - seg * steps;
-    const int left = (int)(g.K - (int64_t)st * TA::kK < TA::kK ? g.K - (int64_t)st * TA::kK : TA::kK);  // K values of this step
-    const char *pa = g.A[PAIR == kTwo ? z : seg] + a_at + (A_KO ? (int64_t)st * TA::kK * g.lda : (int64_t)st * kStepBytes);
+    const int64_t k0 = (int64_t)st * TA::kK, kleft = g.K - k0;
+    const int left = (int)(kleft < TA::kK ? kleft : TA::kK);  // K values of this step
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     {
-      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pa), 0, kRange, 0x00027000);
+      const char *p = g.A[PAIR == kTwo ? z : seg] + (A_KO ? k0 * g.lda + m0 * (int64_t)sizeof(T) : m0 * g.lda + k0 * (int64_t)sizeof(T));
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, range(A_KO ? kleft : g.M - m0, g.lda), 0x00027000);
+      const bool on = A_KO || l.ka < left;
 #pragma unroll
-      for (int q = 0; q < QA; q++)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds_char *)(la + (q * kWaves + wave) * 1024), 16, l.ka[q] < left ? (int)l.a[q] : (int)kNowhere, 0, 0, 0);
+      for (int q = 0; q < QA; q++) {
+        const uint32_t o = kSameA ? l.a[0] + (uint32_t)(q * l.da) : l.a[kSameA ? 0 : q];
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds_char *)(la + (q * kWaves + wave) * 1024), 16, on ? (int)o : (int)kNowhere, 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int half = 0; half < (PAIR == kDual ? 2 : 1); half++) {
-      const char *pb = g.B[PAIR == kDual ? half : seg] + b_at + (B_KO ? (int64_t)st * TB::kK * g.ldb : (int64_t)st * kStepBytes);
-      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pb), 0, kRange, 0x00027000);
-      constexpr int per = PAIR == kDual ? QB / 2 : QB;
+      const char *p = g.B[PAIR == kDual ? half : seg] + (B_KO ? k0 * g.ldb + n0 * (int64_t)sizeof(T) : n0 * g.ldb + k0 * (int64_t)sizeof(T));
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, range(B_KO ? kleft : g.N - n0, g.ldb), 0x00027000);
+      const bool on = B_KO || l.kb < left;
 #pragma unroll
-      for (int q = 0; q < per; q++)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds_char *)(lb + ((half * per + q) * kWaves + wave) * 1024), 16, l.kb[q] < left ? (int)l.b[q] : (int)kNowhere, 0, 0, 0);
+      for (int q = 0; q < PB; q++) {
+        const uint32_t o = kSameB ? l.b[0] + (uint32_t)(q * l.db) : l.b[kSameB ? 0 : q];
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds_char *)(lb + ((half * PB + q) * kWaves + wave) * 1024), 16, on ? (int)o : (int)kNowhere, 0, 0, 0);
+      }
     }
   }
   static __device__ __forceinline__ void compute(const char *la, const char *lb, int wm, int wn, int lane, f32x4 (&acc)[FM][FN]) {
@@ -228,8 +248,8 @@ __device__ __forceinline__ void loads_done() {
   __shared__ __align__(16) char ldsA1[G::TA::kBytes], ldsB1[G::TB::kBytes];
 
 template <typename G>
-__device__ __forceinline__ void gemm_loop(const GemmArgs &g, int m0, int n0, int s0, int s1, int steps, int z, bool a_ko, bool b_ko, size_t elem, char *ldsA0,
-                                          char *ldsB0, char *ldsA1, char *ldsB1, int wm, int wn, int lane, f32x4 (&acc)[G::FM][G::FN]) {
+__device__ __forceinline__ void gemm_loop(const GemmArgs &g, int m0, int n0, int s0, int s1, int steps, int z, char *ldsA0, char *ldsB0,
+                                          char *ldsA1, char *ldsB1, int wm, int wn, int lane, f32x4 (&acc)[G::FM][G::FN]) {
 #pragma unroll
   for (int i = 0; i < G::FM; i++)
 #pragma unroll
@@ -237,15 +257,14 @@ __device__ __forceinline__ void gemm_loop(const GemmArgs &g, int m0, int n0, int
   if (s0 >= s1) return;
   typename G::Load l;
   G::plan(l, g, m0, n0);
-  const int64_t a_at = a_ko ? (int64_t)m0 * (int64_t)elem : (int64_t)m0 * g.lda, b_at = b_ko ? (int64_t)n0 * (int64_t)elem : (int64_t)n0 * g.ldb;
-  G::load(l, g, s0, steps, z, a_at, b_at, ldsA0, ldsB0);
+  G::load(l, g, m0, n0, s0, steps, z, ldsA0, ldsB0);
   loads_done();
   int s = s0;
   for (; s + 1 < s1; s += 2) {  // (no way out in the middle: the sums would be moved between registers there)
-    G::load(l, g, s + 1, steps, z, a_at, b_at, ldsA1, ldsB1);
+    G::load(l, g, m0, n0, s + 1, steps, z, ldsA1, ldsB1);
     G::compute(ldsA0, ldsB0, wm, wn, lane, acc);
     loads_done();
-    if (s + 2 < s1) G::load(l, g, s + 2, steps, z, a_at, b_at, ldsA0, ldsB0);
+    if (s + 2 < s1) G::load(l, g, m0, n0, s + 2, steps, z, ldsA0, ldsB0);
     G::compute(ldsA1, ldsB1, wm, wn, lane, acc);
     loads_done();
   }
