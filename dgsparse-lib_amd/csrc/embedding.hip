@@ -7,7 +7,7 @@
 //
 // Lookup: HBM-bound gather, each row read once in 16-byte pieces.
 // Gradient: positions are sorted by id with the position as the tie-break (dgs_embedding_sort_*), so every row's sum has one fixed order
-// and no atomics.  The sorted list is cut into chunks of `chunk` positions; a group of lanes walks a chunk with a running sum in 32 bits
+// and no atomics.  The sorted list is cut into chunks of 32 or 64 positions; a group of lanes walks a chunk with a running sum in 32 bits
 // and writes each row that lies within its chunk.  A row whose positions cross a chunk's border (a frequent token) leaves partial sums in the
 // workspace, which embedding_join adds up in chunk order.  Rows without a token are cleared by workgroups of the same launch: they find
 // the few ids of their share of the table by binary search in the sorted list, so the table is written once and read never.
@@ -119,8 +119,8 @@ __global__ __launch_bounds__(kSortWaves *kWave) void embedding_place_kernel(int6
   // this thread's digit: positions with it in all workgroups, and in those in front of this one
   int all = 0, front = 0;
   if (t < bins) {
-#pragma unroll 8
-    for (int b = 0; b < (int)gridDim.x; b++) {
+#pragma unroll 16
+    for (int b = 0; b < (int)gridDim.x; b++) {  // (independent reads out of L2: as many as registers take are in flight)
       const int h = hist[(int64_t)b * bins + t];
       all += h;
       front += b < (int)blockIdx.x ? h : 0;
@@ -171,36 +171,44 @@ __global__ __launch_bounds__(kSortWaves *kWave) void embedding_place_kernel(int6
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------------
-// Workgroups [0, fill_blocks): rows without a token.  The others: chunks of the sorted list.  Partial rows: slot 2c for the row that
-// chunk c goes on with from the chunk before, slot 2c + 1 for the row that starts in chunk c and goes on behind it.
+// Where the first key >= `key` stands in the sorted list skey[0, n) of every `stride`-th key: a wave splits the range 64-fold, 3 steps for
+// 2^18 positions.  Every lane of the wave gets the answer in [0, n].
+__device__ __forceinline__ int64_t lower_bound_wave(const uint32_t *__restrict__ skey, int64_t stride, int64_t n, uint32_t key) {
+  const int lane = threadIdx.x & 63;
+  int64_t lo = 0, hi = n;
+  while (hi > lo) {
+    const int64_t step = (hi - lo + kWave - 1) / kWave, at = lo + lane * step;
+    // probes in front of the answer: the first `less` lanes
+    const int less = __popcll(__ballot(at < hi && skey[(at < hi ? at : lo) * stride] < key));
+    const int64_t nlo = less ? lo + (int64_t)(less - 1) * step + 1 : lo, nhi = lo + (int64_t)less * step;
+    hi = nhi < hi ? nhi : hi;
+    lo = nlo;
+  }
+  return lo;
+}
+
+constexpr int kLeastLanes = 8;                 // of a group
+constexpr int kHeld = kBlock / kLeastLanes * 64;  // positions of a workgroup, at most
+
+// Workgroups [0, work): chunks of the sorted list, kBlock / G of them each, `tiles` workgroups for the columns.  Behind them: rows without a
+// token, which stream to memory while the chunks wait for theirs.  Partial rows: slot 2c for the row that chunk c goes on with from the
+// chunk before, slot 2c + 1 for the row that starts in chunk c and goes on behind it.
 template <typename T, bool VECTOR>
-__global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_t V, int D, int G, int chunk, int64_t n_chunks, int64_t fill_blocks, int fill_rows,
+__global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_t V, int D, int G, int chunk, int64_t n_chunks, int tiles, int64_t work, int fill_rows,
                                                                const uint32_t *__restrict__ skey, const int *__restrict__ spos,
                                                                const T *__restrict__ dout, int64_t ldo, float scale, T *__restrict__ dtable,
                                                                float *__restrict__ partial) {
   constexpr int W = kVec<T>;
-  if ((int64_t)blockIdx.x < fill_blocks) {
-    // fill_rows (<= 256) rows from v0.  The sorted list's part with these ids lies between two lower bounds; a wave looks for each by
-    // 64-fold splitting: 3 steps for 2^18 positions.
+  const int t = threadIdx.x, lane = t & (G - 1);
+  if ((int64_t)blockIdx.x >= work) {
+    // fill_rows (<= 256) rows from v0; the sorted list's part with these ids lies between two lower bounds
     __shared__ uint32_t seen[8];
     __shared__ int64_t bound[2];
-    const int64_t v0 = (int64_t)blockIdx.x * fill_rows, v1 = v0 + fill_rows < V ? v0 + fill_rows : V;
-    const int t = threadIdx.x;
+    const int64_t v0 = ((int64_t)blockIdx.x - work) * fill_rows, v1 = v0 + fill_rows < V ? v0 + fill_rows : V;
     if (t < 8) seen[t] = 0u;
     if (t < 2 * kWave) {
-      const int lane = t & 63;
-      const uint32_t key = (uint32_t)(t < kWave ? v0 : v1);
-      int64_t lo = 0, hi = n;  // the answer lies in [lo, hi]
-      while (hi > lo) {
-        const int64_t step = (hi - lo + kWave - 1) / kWave;
-        const int64_t at = lo + lane * step;
-        const int less = __popcll(__ballot(at < hi && skey[at < hi ? at : lo] < key));  // probes in front of the bound: the first `less` lanes
-        const int64_t nlo = less ? lo + (int64_t)(less - 1) * step + 1 : lo;
-        const int64_t nhi = lo + (int64_t)less * step;
-        hi = nhi < hi ? nhi : hi;
-        lo = nlo;
-      }
-      if (lane == 0) bound[t / kWave] = lo;
+      const int64_t at = lower_bound_wave(skey, 1, n, (uint32_t)(t < kWave ? v0 : v1));
+      if ((t & 63) == 0) bound[t / kWave] = at;
     }
     __syncthreads();
     for (int64_t q = bound[0] + t; q < bound[1]; q += kBlock) {
@@ -211,7 +219,6 @@ __global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_
     float zero[W];
 #pragma unroll
     for (int k = 0; k < W; k++) zero[k] = 0.0f;
-    const int lane = t & (G - 1);
     for (int64_t v = v0 + t / G; v < v1; v += kBlock / G) {
       const int r = (int)(v - v0);
       if ((seen[r >> 5] >> (r & 31)) & 1) continue;
@@ -219,52 +226,54 @@ __global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_
     }
     return;
   }
-  const int lane = threadIdx.x & (G - 1);
-  const int64_t ch = ((int64_t)blockIdx.x - fill_blocks) * (kBlock / G) + threadIdx.x / G;
-  if (ch >= n_chunks) return;
-  const int64_t q0 = ch * chunk, q1 = q0 + chunk < n ? q0 + chunk : n;
-  const int c = ((int)blockIdx.y * G + lane) * W;
-  if (c >= D) return;
-  bool head = ch > 0 && skey[q0 - 1] == skey[q0];  // the first row goes on from the chunk before
+  // the workgroup's keys (with one neighbour at either end) and positions, read once
+  __shared__ uint32_t key[kHeld + 2];
+  __shared__ int pos[kHeld];
+  const int64_t wb = (int64_t)blockIdx.x / tiles, p0 = wb * (kBlock / G) * chunk;
+  const int held = (int)(n - p0 < (int64_t)(kBlock / G) * chunk ? n - p0 : (int64_t)(kBlock / G) * chunk);
+  for (int i = t; i < held + 2; i += kBlock) {
+    const int64_t q = p0 + i - 1;
+    key[i] = q >= 0 && q < n ? skey[q] : 0xffffffffu;  // (no key: keys are at most V)
+    if (i < held) pos[i] = spos[p0 + i];
+  }
+  __syncthreads();
+  const int64_t ch = wb * (kBlock / G) + t / G;
+  const int c = ((int)((int64_t)blockIdx.x % tiles) * G + lane) * W;
+  if (ch >= n_chunks || c >= D) return;
+  const int q0 = t / G * chunk, q1 = q0 + chunk < held ? q0 + chunk : held;
+  bool head = key[q0] == key[q0 + 1];  // the first row goes on from the chunk before
   float acc[W];
 #pragma unroll
   for (int k = 0; k < W; k++) acc[k] = 0.0f;
-  uint32_t key = skey[q0];
-  constexpr int U = 4;  // rows in flight
-  for (int64_t q = q0; q < q1; q += U) {
+  constexpr int U = 8;  // rows in flight
+  for (int q = q0; q < q1; q += U) {
     float x[U][W];
-    uint32_t kk[U + 1];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int64_t at = q + u < q1 ? q + u : q1 - 1;
-      kk[u] = skey[at];
-      if (kk[u] < (uint32_t)V) load_row<T, VECTOR>(dout + (int64_t)spos[at] * ldo, c, D, x[u]);
+      const int at = q + u < q1 ? q + u : q1 - 1;
+      if (key[at + 1] < (uint32_t)V) load_row<T, VECTOR>(dout + (int64_t)pos[at] * ldo, c, D, x[u]);
     }
-    kk[U] = q + U < n ? skey[q + U] : 0xffffffffu;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if (q + u >= q1 || kk[u] >= (uint32_t)V) break;
-      key = kk[u];
+      const uint32_t now = key[(q + u < q1 ? q + u : q1 - 1) + 1];
+      if (q + u >= q1 || now >= (uint32_t)V) break;  // (ids that add to no row come last)
 #pragma unroll
       for (int k = 0; k < W; k++) acc[k] += x[u][k];
-      const bool last = q + u + 1 >= q1;                                     // of the chunk
-      const uint32_t next = last ? (q1 < n ? skey[q1] : 0xffffffffu) : kk[u + 1];
-      if (next != key || last) {
-        const bool on = next == key;  // the row goes on in the next chunk
-        if (head || on) {
-          float *slot = partial + (2 * ch + (head ? 0 : 1)) * (int64_t)D;
+      const bool on = key[q + u + 2] == now;  // the row goes on behind this position
+      if (on && q + u + 1 < q1) continue;
+      if (head || on) {
+        float *slot = partial + (2 * ch + (head ? 0 : 1)) * (int64_t)D;
 #pragma unroll
-          for (int k = 0; k < W; k++)
-            if (c + k < D) slot[c + k] = acc[k];
-        } else {
+        for (int k = 0; k < W; k++)
+          if (c + k < D) slot[c + k] = acc[k];
+      } else {
 #pragma unroll
-          for (int k = 0; k < W; k++) acc[k] *= scale;
-          store_row<T, VECTOR>(dtable + (int64_t)key * D, c, D, acc);
-        }
-        head = false;
-#pragma unroll
-        for (int k = 0; k < W; k++) acc[k] = 0.0f;
+        for (int k = 0; k < W; k++) acc[k] *= scale;
+        store_row<T, VECTOR>(dtable + (int64_t)now * D, c, D, acc);
       }
+      head = false;
+#pragma unroll
+      for (int k = 0; k < W; k++) acc[k] = 0.0f;
     }
   }
 }
@@ -277,17 +286,13 @@ __global__ __launch_bounds__(kBlock) void embedding_join_kernel(int64_t n, int64
   const int64_t b = (int64_t)blockIdx.x + 1;
   const int64_t at = b * chunk;
   const uint32_t key = skey[at];
-  if (key >= (uint32_t)V || skey[at - 1] != key) return;
-  if (b > 1 && skey[at - chunk - 1] == key) return;  // an earlier border owns the row
+  const uint32_t prev = skey[at - 1], start = b > 1 ? skey[at - chunk - 1] : 0xffffffffu;
+  if (key >= (uint32_t)V || prev != key || start == key) return;  // (start == key: an earlier border owns the row)
   __shared__ int64_t end;
   __shared__ float sum[8][32];
-  if (threadIdx.x == 0) {  // the last chunk that begins within the row: binary search over the chunks' first keys
-    int64_t lo = b, hi = n_chunks - 1;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) / 2;
-      if (skey[mid * chunk] == key) lo = mid; else hi = mid - 1;
-    }
-    end = lo;
+  if (threadIdx.x < kWave) {  // the last chunk that begins within the row, by the chunks' first keys
+    const int64_t behind = b + lower_bound_wave(skey + at, chunk, n_chunks - b, key + 1);
+    if (threadIdx.x == 0) end = behind - 1;
   }
   __syncthreads();
   const int col = threadIdx.x & 31, sub = threadIdx.x >> 5;
@@ -299,10 +304,11 @@ __global__ __launch_bounds__(kBlock) void embedding_join_kernel(int64_t n, int64
     if (c < D) {
       if (sub == 0) a = partial[(2 * (b - 1) + 1) * (int64_t)D + c];
       int64_t k = lo;
-      for (; k + 3 < hi; k += 4) {
-        const float p0 = partial[2 * k * (int64_t)D + c], p1 = partial[2 * (k + 1) * (int64_t)D + c], p2 = partial[2 * (k + 2) * (int64_t)D + c],
-                    p3 = partial[2 * (k + 3) * (int64_t)D + c];
-        a += (p0 + p1) + (p2 + p3);
+      for (; k + 7 < hi; k += 8) {
+        float p[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) p[u] = partial[2 * (k + u) * (int64_t)D + c];
+        a += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       }
       for (; k < hi; k++) a += partial[2 * k * (int64_t)D + c];
     }
@@ -329,7 +335,7 @@ static int key_bits(int64_t V) {  // keys 0 .. V
   return b;
 }
 // Positions a chunk: enough chunks for the card, and for very long lists few enough that a frequent token's partial sums stay few.
-static int chunk_of(int64_t n) { return n <= (1 << 20) ? 32 : 256; }
+static int chunk_of(int64_t n) { return n <= (1 << 20) ? 32 : 64; }
 
 struct SortPlan {
   int passes, bits, tile;
@@ -409,24 +415,18 @@ static int bwd(int64_t n, int64_t V, int64_t D, const uint32_t *key, const int *
                hipStream_t st) {
   const bool vec = D % kVec<T> == 0 && ldo % kVec<T> == 0 && aligned_to(dout, 16) && aligned_to(dtable, 16);
   const int64_t vecs = (D + kVec<T> - 1) / kVec<T>;
-  const int G = lanes_for(vecs), chunk = chunk_of(n);
-  const int64_t n_chunks = (n + chunk - 1) / chunk, per = kBlock / G;
+  const int G = lanes_for(vecs) < kLeastLanes ? kLeastLanes : lanes_for(vecs), chunk = chunk_of(n);
+  const int64_t n_chunks = (n + chunk - 1) / chunk, per = kBlock / G, tiles = (vecs + G - 1) / G;
   // a clearing workgroup writes about 64 KB; its rows go by a bit map of 256
   const int64_t rowb = D * (int64_t)sizeof(T);
   const int fill_rows = (int)(65536 / rowb < 1 ? 1 : 65536 / rowb > 256 ? 256 : 65536 / rowb);
-  const int64_t fill = (V + fill_rows - 1) / fill_rows, work = (n_chunks + per - 1) / per;
+  const int64_t fill = (V + fill_rows - 1) / fill_rows, work = (n_chunks + per - 1) / per * tiles;
   if (fill + work > INT32_MAX) return DGS_ERANGE;
-  const int64_t tiles = (vecs + G - 1) / G;
-  if (tiles > 65535) return DGS_ERANGE;
-  // (the clearing part of a launch with several column tiles runs in the first of them alone)
-  for (int part = 0; part < (tiles > 1 ? 2 : 1); part++) {
-    const int64_t f = tiles > 1 && part ? 0 : fill, w = tiles > 1 && !part ? 0 : work;
-    const dim3 grid((unsigned)(f + w), (unsigned)(tiles > 1 && !part ? 1 : tiles));
-    if (vec)
-      hipLaunchKernelGGL((embedding_bwd_kernel<T, true>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, f, fill_rows, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
-    else
-      hipLaunchKernelGGL((embedding_bwd_kernel<T, false>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, f, fill_rows, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
-  }
+  const dim3 grid((unsigned)(work + fill));
+  if (vec)
+    hipLaunchKernelGGL((embedding_bwd_kernel<T, true>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, (int)tiles, work, fill_rows, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
+  else
+    hipLaunchKernelGGL((embedding_bwd_kernel<T, false>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, (int)tiles, work, fill_rows, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
   if (check_launch() != DGS_OK) return DGS_ELAUNCH;
   if (n_chunks > 1) {
     const int64_t cols = (D + 31) / 32;

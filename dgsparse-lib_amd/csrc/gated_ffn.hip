@@ -2,8 +2,9 @@
 //
 //   forward    g = x Wg^T, u = x Wu^T side by side in one tile (kDual: a wave holds the g and the u of the same columns), h = act(g) u where
 //              the tile's sums leave the registers: g and u never reach memory.
-//   backward   the forward's products are made again (4 rows D F flops, instead of keeping 8 bytes for each value of h), and where they
-//              leave the registers  dg = dh u act'(g), du = dh act(g), rounded once to the type: the operands of the other products,
+//   backward   dg = dh u act'(g), du = dh act(g), rounded once to the type: the operands of the other products.  g and u are those that the
+//              forward pass kept (8 bytes for each value of h, one pass over them), or they are made again (4 rows D F flops) and dg, du
+//              formed where they leave the registers.
 //              dx = dg Wg + du Wu  (one walk over 2 F),  dWg = dg^T x, dWu = du^T x  (sums over the rows, split where there are few tiles).
 //
 // Bound: the matrix cores (12 rows D F flops forward and backward, 16 with the products made again); for few rows the weights' bytes
@@ -32,12 +33,13 @@ __device__ __forceinline__ float act(float g, float &d) {
 
 struct GatedOut {
   const void *dh;   // backward: [M, F], contiguous
+  float *pre;       // forward: where the two products are kept, [2][M, F], or null
   void *o0, *o1;    // forward: h; backward: dg, du
   int64_t F, ldo;   // columns of h / dh; row stride of the outputs (backward: the padded columns F .. ldo are written too, as zeros)
 };
 
 template <typename T, int ACT, bool BWD>
-__device__ __forceinline__ void gated_store(const GatedOut &o, int64_t m, int64_t n, const f32x4 &g, const f32x4 &u, bool vec) {
+__device__ __forceinline__ void gated_store(const GatedOut &o, int64_t M, int64_t m, int64_t n, const f32x4 &g, const f32x4 &u, bool vec) {
   f32x4 a, b;
   if constexpr (BWD) {
     const f32x4 dh = n < o.F ? load4<T>((const T *)o.dh + m * o.F + n, o.F - n, o.F % 4 == 0) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -58,6 +60,10 @@ __device__ __forceinline__ void gated_store(const GatedOut &o, int64_t m, int64_
       a[k] = act<ACT>(g[k], d) * u[k];
     }
     store4<T>((T *)o.o0 + m * o.ldo + n, a, o.F - n, vec);
+    if (o.pre) {
+      store4<float>(o.pre + m * o.F + n, g, o.F - n, vec);
+      store4<float>(o.pre + (M + m) * o.F + n, u, o.F - n, vec);
+    }
   }
 }
 
@@ -80,8 +86,35 @@ __global__ __launch_bounds__(64 * WM *WN) void gated_kernel(const GemmArgs g, co
 #pragma unroll
     for (int j = 0; j < G::FN / 2; j++) {
       const int64_t n = n0 + G::c_col(wn, j) + 4 * (lane >> 4);
-      if (n < end) gated_store<T, ACT, BWD>(o, m, n, acc[i][j], acc[i][j + G::FN / 2], vec);
+      if (n < end) gated_store<T, ACT, BWD>(o, g.M, m, n, acc[i][j], acc[i][j + G::FN / 2], vec);
     }
+  }
+}
+
+// dg and du from kept products: one pass over them and dh.  G lanes a row; the outputs' padding (F .. ldo) gets zeros.
+template <typename T, int ACT, bool VECTOR>
+__global__ __launch_bounds__(kBlock) void gated_split_kernel(int64_t M, int G, const GatedOut o) {
+  constexpr int V = kVec<T>;
+  const int lane = threadIdx.x & (G - 1);
+  const int64_t m = (int64_t)blockIdx.x * (kBlock / G) + threadIdx.x / G;
+  if (m >= M) return;
+  const int F = (int)o.F;
+  for (int c = lane * V; c < F; c += G * V) {
+    float dh[V], a[V], b[V];
+    load_row<T, VECTOR>((const T *)o.dh + m * o.F, c, F, dh);
+#pragma unroll
+    for (int q = 0; q < V; q += 4) {
+      const f32x4 g = load4<float>(o.pre + m * o.F + c + q, F - c - q, VECTOR), u = load4<float>(o.pre + (M + m) * o.F + c + q, F - c - q, VECTOR);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        float d;
+        const float v = act<ACT>(g[k], d);  // (behind F: dh = 0 and finite others)
+        a[q + k] = dh[q + k] * u[k] * d;
+        b[q + k] = dh[q + k] * v;
+      }
+    }
+    store_row<T, true>((T *)o.o0 + m * o.ldo, c, F, a);  // (their rows are whole 16-byte pieces)
+    store_row<T, true>((T *)o.o1 + m * o.ldo, c, F, b);
   }
 }
 
@@ -89,7 +122,8 @@ __global__ __launch_bounds__(64 * WM *WN) void gated_kernel(const GemmArgs g, co
 // instructions (128 bytes of each of 16 rows a wave at a time); x comes out of L2.  The waves' sums meet in LDS.
 template <typename T, int FM, int ACT>
 __global__ __launch_bounds__(512) void gated_few_kernel(const char *__restrict__ x, int64_t ldx, const char *__restrict__ wg, const char *__restrict__ wu, int64_t ldw,
-                                                        int M, int64_t F, int64_t kbytes, T *__restrict__ h) {
+                                                        int M, int64_t F, int64_t kbytes, T *__restrict__ h,
+                                                        float *__restrict__ pre) {
   constexpr int kW = 8;
   __shared__ float sum[kW][2][16 * FM][17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -146,6 +180,10 @@ __global__ __launch_bounds__(512) void gated_few_kernel(const char *__restrict__
       u += sum[w][1][m][c];
     }
     h[(int64_t)m * F + n0 + c] = from_f32<T>(act<ACT>(g, d) * u);
+    if (pre) {
+      pre[(int64_t)m * F + n0 + c] = g;
+      pre[(int64_t)(M + m) * F + n0 + c] = u;
+    }
   }
 }
 
@@ -227,7 +265,7 @@ template <typename T>
 static int operands(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, char *ws, const Layout &L, hipStream_t st,
                     Operands<T> &o) {
   if (!L.pad) {
-    if (!rows16(x, D, ldx, sizeof(T)) || !rows16(wg, D, ldw, sizeof(T)) || !rows16(wu, D, ldw, sizeof(T))) return DGS_EINVAL;
+    if (!rows16(x, D, ldx, sizeof(T)) || !rows16(wg, D, ldw, sizeof(T)) || !rows16(wu, D, ldw, sizeof(T)) || ldx < D || ldw < D) return DGS_EINVAL;
     o = {(const char *)x, (const char *)wg, (const char *)wu, ldx, ldw};
     return DGS_OK;
   }
@@ -288,7 +326,7 @@ static int launch_product(GemmArgs g, PlainOut o, const TilePlan &p, float *part
 constexpr int64_t kFewRows = 64;
 
 template <typename T, int ACT>
-static int ffn_fwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, void *h, char *ws, hipStream_t st) {
+static int ffn_fwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, void *h, float *pre, char *ws, hipStream_t st) {
   const Layout L = layout<T>(rows, D, F, false, ldx);
   Operands<T> op;
   const int rc = operands<T>(rows, D, F, x, ldx, wg, wu, ldw, ws, L, st, op);
@@ -296,20 +334,20 @@ static int ffn_fwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ld
   if (rows <= kFewRows) {
     const dim3 grid((unsigned)((F + 15) / 16));
     const int64_t kb = (int64_t)(L.pad ? L.ldx : D) * (int64_t)sizeof(T), lx = op.ldx * (int64_t)sizeof(T), lw = op.ldw * (int64_t)sizeof(T);
-#define DGS_FEW(FM_) hipLaunchKernelGGL((gated_few_kernel<T, FM_, ACT>), grid, dim3(512), 0, st, op.x, lx, op.wg, op.wu, lw, (int)rows, F, kb, (T *)h)
+#define DGS_FEW(FM_) hipLaunchKernelGGL((gated_few_kernel<T, FM_, ACT>), grid, dim3(512), 0, st, op.x, lx, op.wg, op.wu, lw, (int)rows, F, kb, (T *)h, pre)
     if (rows <= 16) DGS_FEW(1);
     else if (rows <= 32) DGS_FEW(2);
     else DGS_FEW(4);
 #undef DGS_FEW
     return check_launch();
   }
-  const GatedOut out = {nullptr, h, nullptr, F, F};
+  const GatedOut out = {nullptr, pre, h, nullptr, F, F};
   return launch_gated<T, ACT, false>(rows, D, F, op, out, st);
 }
 
 template <typename T, int ACT>
-static int ffn_bwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, const void *dh, void *dx, void *dwg, void *dwu,
-                   char *ws, hipStream_t st) {
+static int ffn_bwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, const float *pre, const void *dh, void *dx, void *dwg,
+                   void *dwu, char *ws, hipStream_t st) {
   const Layout L = layout<T>(rows, D, F, true, ldx);
   Operands<T> op;
   int rc = operands<T>(rows, D, F, x, ldx, wg, wu, ldw, ws, L, st, op);
@@ -317,8 +355,19 @@ static int ffn_bwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ld
   constexpr int64_t size = sizeof(T);
   constexpr int kK = kStepBytes / (int)sizeof(T);
   char *dg = ws + L.dg, *du = ws + L.du;
-  const GatedOut out = {dh, dg, du, F, L.ldg};
-  rc = launch_gated<T, ACT, true>(rows, D, F, op, out, st);
+  const GatedOut out = {dh, const_cast<float *>(pre), dg, du, F, L.ldg};
+  if (pre) {
+    int G = 1;
+    while (G < kBlock && G * kVec<T> < F) G <<= 1;
+    const dim3 grid((unsigned)((rows + kBlock / G - 1) / (kBlock / G)));
+    if (F % kVec<T> == 0)
+      hipLaunchKernelGGL((gated_split_kernel<T, ACT, true>), grid, dim3(kBlock), 0, st, rows, G, out);
+    else
+      hipLaunchKernelGGL((gated_split_kernel<T, ACT, false>), grid, dim3(kBlock), 0, st, rows, G, out);
+    rc = check_launch();
+  } else {
+    rc = launch_gated<T, ACT, true>(rows, D, F, op, out, st);
+  }
   float *partial = (float *)(ws + L.partial);
   if (rc == DGS_OK && dx) {  // dx [rows, D] = dg Wg + du Wu: K = F, the weights K-outer
     GemmArgs g = {{dg, du}, {op.wg, op.wu}, L.ldg * size, op.ldw * size, rows, D, F, 0, 0, 1};
@@ -359,16 +408,16 @@ extern "C" size_t dgs_gated_ffn_workspace_bytes(int dtype, int64_t rows, int64_t
   }
 
 extern "C" int dgs_gated_ffn(int dtype, int activation, int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *w_gate, const void *w_up, int64_t ldw,
-                             void *h, void *workspace, size_t workspace_bytes, dgsStream_t stream) {
+                             void *h, float *pre, void *workspace, size_t workspace_bytes, dgsStream_t stream) {
   const int rc = ffn_sizes(dtype, activation, rows, D, F, ldx, ldw);
   if (rc != DGS_OK) return rc;
   if (rows == 0) return DGS_OK;
-  if (!x || !w_gate || !w_up || !h || !aligned_to(h, 16)) return DGS_EINVAL;
+  if (!x || !w_gate || !w_up || !h || !aligned_to(h, 16) || !aligned_to(pre, 16)) return DGS_EINVAL;
   const size_t need = dgs_gated_ffn_workspace_bytes(dtype, rows, D, F, 0);
   if (need && (!workspace || workspace_bytes < need)) return DGS_EWORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   char *ws = static_cast<char *>(workspace);
-#define ARGS (rows, D, F, x, ldx, w_gate, w_up, ldw, h, ws, st)
+#define ARGS (rows, D, F, x, ldx, w_gate, w_up, ldw, h, pre, ws, st)
   if (dtype == DGS_F32) DGS_ACTS(float, ffn_fwd)
   if (dtype == DGS_F16) DGS_ACTS(f16, ffn_fwd)
   DGS_ACTS(bf16, ffn_fwd)
@@ -376,16 +425,16 @@ extern "C" int dgs_gated_ffn(int dtype, int activation, int64_t rows, int64_t D,
 }
 
 extern "C" int dgs_gated_ffn_bwd(int dtype, int activation, int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *w_gate, const void *w_up, int64_t ldw,
-                                 const void *dh, void *dx, void *dw_gate, void *dw_up, void *workspace, size_t workspace_bytes, dgsStream_t stream) {
+                                 const float *pre, const void *dh, void *dx, void *dw_gate, void *dw_up, void *workspace, size_t workspace_bytes, dgsStream_t stream) {
   const int rc = ffn_sizes(dtype, activation, rows, D, F, ldx, ldw);
   if (rc != DGS_OK) return rc;
-  if (rows == 0 || !x || !w_gate || !w_up || !dh || !dw_gate != !dw_up || !aligned_to(dh, 16) || !aligned_to(dx, 16) || !aligned_to(dw_gate, 16) || !aligned_to(dw_up, 16))
+  if (rows == 0 || !x || !w_gate || !w_up || !dh || !dw_gate != !dw_up || !aligned_to(dh, 16) || !aligned_to(dx, 16) || !aligned_to(dw_gate, 16) || !aligned_to(dw_up, 16) || !aligned_to(pre, 16))
     return DGS_EINVAL;
   const size_t need = dgs_gated_ffn_workspace_bytes(dtype, rows, D, F, 1);
   if (!workspace || workspace_bytes < need) return DGS_EWORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   char *ws = static_cast<char *>(workspace);
-#define ARGS (rows, D, F, x, ldx, w_gate, w_up, ldw, dh, dx, dw_gate, dw_up, ws, st)
+#define ARGS (rows, D, F, x, ldx, w_gate, w_up, ldw, pre, dh, dx, dw_gate, dw_up, ws, st)
   if (dtype == DGS_F32) DGS_ACTS(float, ffn_bwd)
   if (dtype == DGS_F16) DGS_ACTS(f16, ffn_bwd)
   DGS_ACTS(bf16, ffn_bwd)

@@ -252,26 +252,36 @@ FfnIn ffn_in(const Tensor &x_, const Tensor &wg_, const Tensor &wu_) {
   }
   return i;
 }
-Tensor ffn_fwd(const Tensor &x, const Tensor &wg, const Tensor &wu, int64_t activation) {
-  ffn_check(x, wg, wu, activation);
+// Whether the forward pass keeps the two products in 32 bits for the backward pass, where the caller leaves it open (keep < 0).  Kept they cost
+// 16 bytes of memory traffic for each value of h, made again 4 D flops: on MI355X even at D = 1024 in 16 bits (1.1 PFLOP/s against
+// 5 TB/s) and 128 in 32 (0.15 PFLOP/s).  Beyond 1 GiB of them they are made again, so that a deep model's activations stay its own.
+bool ffn_keeps(const Tensor &x, const Tensor &wg, int64_t keep) {
+  if (keep >= 0) return keep != 0;
+  const int64_t D = x.size(-1), count = x.numel() / D * wg.size(0);
+  return D >= (x.element_size() == 4 ? 256 : 1024) && count <= (int64_t(1) << 27);
+}
+Tensor ffn_fwd(const Tensor &x, const Tensor &wg, const Tensor &wu, int64_t activation, Tensor *pre = nullptr) {
   const Guard guard(x.device());
   auto shape = x.sizes().vec();
   shape.back() = wg.size(0);
   Tensor h = at::empty(shape, x.options());
   if (h.numel() == 0) return h;
   const FfnIn i = ffn_in(x, wg, wu);
+  if (pre) *pre = at::empty({2, i.rows, i.F}, x.options().dtype(at::kFloat));
   const size_t wsb = dgs_gated_ffn_workspace_bytes(i.dtype, i.rows, i.D, i.F, 0);
   Tensor ws = wsb ? workspace(wsb, x) : Tensor();
   check_rc(dgs_gated_ffn(i.dtype, (int)activation, i.rows, i.D, i.F, i.x.data_ptr(), i.ldx, i.wg.data_ptr(), i.wu.data_ptr(), i.ldw, h.data_ptr(),
-                         wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
+                         pre ? pre->data_ptr<float>() : nullptr, wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
            "gated_ffn");
   return h;
 }
 struct GatedFfn : public torch::autograd::Function<GatedFfn> {
-  static Tensor forward(AutogradContext *ctx, Tensor x, Tensor wg, Tensor wu, int64_t activation) {
-    ctx->save_for_backward({x, wg, wu});
+  static Tensor forward(AutogradContext *ctx, Tensor x, Tensor wg, Tensor wu, int64_t activation, int64_t keep) {
+    Tensor pre;
+    Tensor h = ffn_fwd(x, wg, wu, activation, ffn_keeps(x, wg, keep) && x.numel() ? &pre : nullptr);
+    ctx->save_for_backward({x, wg, wu, pre});
     ctx->saved_data["act"] = activation;
-    return ffn_fwd(x, wg, wu, activation);
+    return h;
   }
   static tensor_list backward(AutogradContext *ctx, tensor_list grads) {
     once("gated_ffn");
@@ -286,22 +296,23 @@ struct GatedFfn : public torch::autograd::Function<GatedFfn> {
         dwg.zero_();
         dwu.zero_();
       }
-      return {dx, dwg, dwu, Tensor()};
+      return {dx, dwg, dwu, Tensor(), Tensor()};
     }
     const FfnIn i = ffn_in(x, wg, wu);
     const Tensor dh = aligned_contiguous(grads[0]);
     const size_t wsb = dgs_gated_ffn_workspace_bytes(i.dtype, i.rows, i.D, i.F, 1);
     Tensor ws = workspace(wsb, x);
     check_rc(dgs_gated_ffn_bwd(i.dtype, (int)ctx->saved_data["act"].toInt(), i.rows, i.D, i.F, i.x.data_ptr(), i.ldx, i.wg.data_ptr(), i.wu.data_ptr(), i.ldw,
-                               dh.data_ptr(), need_x ? dx.data_ptr() : nullptr, need_w ? dwg.data_ptr() : nullptr, need_w ? dwu.data_ptr() : nullptr,
+                               saved[3].defined() ? saved[3].data_ptr<float>() : nullptr, dh.data_ptr(), need_x ? dx.data_ptr() : nullptr, need_w ? dwg.data_ptr() : nullptr, need_w ? dwu.data_ptr() : nullptr,
                                ws.data_ptr(), wsb, cur_stream()),
              "gated_ffn backward");
-    return {dx, dwg, dwu, Tensor()};
+    return {dx, dwg, dwu, Tensor(), Tensor()};
   }
 };
-Tensor gated_ffn_op(Tensor x, Tensor wg, Tensor wu, int64_t activation) {
+Tensor gated_ffn_op(Tensor x, Tensor wg, Tensor wu, int64_t activation, int64_t keep) {
+  ffn_check(x, wg, wu, activation);
   if (!(at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad()))) return ffn_fwd(x, wg, wu, activation);
-  return GatedFfn::apply(x, wg, wu, activation);
+  return GatedFfn::apply(x, wg, wu, activation, keep);
 }
 
 // ---- 8 bits ----------------------------------------------------------------------------------------------------------------

@@ -46,15 +46,17 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
 _ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
 
 
-def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = 'silu') -> torch.Tensor:
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = 'silu',
+              recompute: Optional[bool] = None) -> torch.Tensor:
     r"""``act(x @ w_gate.T) * (x @ w_up.T)`` in one kernel: both projections of a gated feed-forward block, the activation (``'silu'``, ``'gelu'``
     in its erf form, or ``'relu'``) and the product.  ``x`` [..., features], the weights [hidden, features] as ``torch.nn.Linear`` keeps them.
 
-    Gradients of ``x`` and both weights.  The backward pass makes the two projections again instead of keeping them, and rounds the two
-    pre-activation gradients once to the operands' type."""
+    Gradients of ``x`` and both weights; the two projections' gradients are rounded once to the operands' type.  For them the backward pass
+    needs the projections: ``recompute=False`` keeps both in 32 bits, ``True`` makes them again, ``None`` keeps them where that is faster
+    and takes no more than 1 GiB.  Both ways give results within the rounding of the other (the same bits from 65 rows on)."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f'dgsparse: activation must be one of {sorted(_ACTIVATIONS)}, not {activation!r}')
-    return torch.ops.dgsparse_spmm.gated_ffn(x, w_gate, w_up, _ACTIVATIONS[activation])
+    return torch.ops.dgsparse_spmm.gated_ffn(x, w_gate, w_up, _ACTIVATIONS[activation], -1 if recompute is None else int(not recompute))
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:

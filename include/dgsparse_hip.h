@@ -460,16 +460,17 @@ int dgs_rms_norm_bwd(int dtype, int64_t rows, int64_t D, const void *s, const vo
 
 /* Gated feed-forward product: h [rows, F] = act(x Wg^T) * (x Wu^T);  x [rows, D] with row distance ldx, Wg and Wu [F, D] with row distance
  * ldw, h contiguous and 16-byte aligned.  Where D is a multiple of 16 bytes, x, Wg and Wu have to lie at multiples of 16 bytes with row
- * distances that are such too (else DGS_EINVAL); any other D is taken through padded copies in the workspace. */
+ * distances that are such too (else DGS_EINVAL); any other D is taken through padded copies in the workspace.
+ * pre (may be null): the two products, [2][rows, F] in 32 bits, 16-byte aligned, for the backward pass. */
 enum { DGS_ACT_SILU = 0, DGS_ACT_GELU = 1, DGS_ACT_RELU = 2 }; /* gelu: with the normal distribution (erf), not its tanh form */
 size_t dgs_gated_ffn_workspace_bytes(int dtype, int64_t rows, int64_t D, int64_t F, int backward);
 int dgs_gated_ffn(int dtype, int activation, int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *w_gate,
-                  const void *w_up, int64_t ldw, void *h, void *workspace, size_t workspace_bytes, dgsStream_t stream);
+                  const void *w_up, int64_t ldw, void *h, float *pre, void *workspace, size_t workspace_bytes, dgsStream_t stream);
 /* Its backward pass, from dh [rows, F]: with g, u the two products, dg = dh u act'(g) and du = dh act(g) (rounded to the type: operands of
- * the matrix cores), dx [rows, D] = dg Wg + du Wu (may be null), dWg = dg^T x and dWu = du^T x [F, D] (both or neither may be null).
+ * the matrix cores; the two products as the forward pass kept them in pre, or, pre null, made again), dx [rows, D] = dg Wg + du Wu (may be null), dWg = dg^T x and dWu = du^T x [F, D] (both or neither may be null).
  * rows > 0; dh and the outputs contiguous, 16-byte aligned. */
 int dgs_gated_ffn_bwd(int dtype, int activation, int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *w_gate,
-                      const void *w_up, int64_t ldw, const void *dh, void *dx, void *dw_gate, void *dw_up, void *workspace,
+                      const void *w_up, int64_t ldw, const float *pre, const void *dh, void *dx, void *dw_gate, void *dw_up, void *workspace,
                       size_t workspace_bytes, dgsStream_t stream);
 
 /* x [rows, cols] in 8-bit floating point (e4m3): q [rows, cols] contiguous, scales [ceil(rows / block_rows), ceil(cols / 128)], one for each

@@ -330,6 +330,11 @@ def check_ffn(x, wg, wu, name, seed=0, dh=None):
     want = ffn_want(x.detach().reshape(-1, D), wg.detach(), wu.detach(), dh.reshape(-1, F), name)
     for k, v in dict(h=h.reshape(-1, F), dx=dx.reshape(-1, D), dw_gate=dwg, dw_up=dwu).items():
         within(v, *want[k], what=k)
+    # the projections kept, or made again: both ways on each case
+    for again in (False, True):
+        h2 = dgsparse.gated_ffn(*leaves, activation=name, recompute=again)
+        for k, v in zip(('h', 'dx', 'dw_gate', 'dw_up'), (h2,) + torch.autograd.grad(h2, leaves, dh)):
+            within(v.reshape(want[k][0].shape), *want[k], what=f'{k} recompute={again}')
     assert torch.equal(h, dgsparse.gated_ffn(x.detach(), wg.detach(), wu.detach(), name))
     return h, dx, dwg, dwu
 
