@@ -194,7 +194,7 @@ constexpr int kHeld = kBlock / kLeastLanes * 64;  // positions of a workgroup, a
 // token, which stream to memory while the chunks wait for theirs.  Partial rows: slot 2c for the row that chunk c goes on with from the
 // chunk before, slot 2c + 1 for the row that starts in chunk c and goes on behind it.
 template <typename T, bool VECTOR>
-__global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_t V, int D, int G, int chunk, int64_t n_chunks, int tiles, int64_t work, int fill_rows,
+__global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_t V, int D, int G, int chunk, int64_t n_chunks, int tiles, int64_t work, int fill_rows, int keep,
                                                                const uint32_t *__restrict__ skey, const int *__restrict__ spos,
                                                                const T *__restrict__ dout, int64_t ldo, float scale, T *__restrict__ dtable,
                                                                float *__restrict__ partial) {
@@ -222,7 +222,11 @@ __global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_
     for (int64_t v = v0 + t / G; v < v1; v += kBlock / G) {
       const int r = (int)(v - v0);
       if ((seen[r >> 5] >> (r & 31)) & 1) continue;
-      for (int c = lane * W; c < D; c += G * W) store_row_stream<T, VECTOR>(dtable + v * (int64_t)D, c, D, zero);
+      if (keep) {
+        for (int c = lane * W; c < D; c += G * W) store_row<T, VECTOR>(dtable + v * (int64_t)D, c, D, zero);
+      } else {
+        for (int c = lane * W; c < D; c += G * W) store_row_stream<T, VECTOR>(dtable + v * (int64_t)D, c, D, zero);
+      }
     }
     return;
   }
@@ -280,16 +284,16 @@ __global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_
 
 // Border b between chunks b - 1 and b: the workgroups of the row that starts in chunk b - 1 and goes on in chunk b add up its partial
 // sums: the start's, then one of each chunk up to the last.  32 columns x 8 shares of the chunks; the shares' sums are joined in order.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void embedding_join_kernel(int64_t n, int64_t V, int D, int chunk, int64_t n_chunks, const uint32_t *__restrict__ skey,
+template <typename T, int V>  // V columns a lane: 4, or 1 where a row of partial sums is no multiple of 16 bytes
+__global__ __launch_bounds__(kBlock) void embedding_join_kernel(int64_t n, int64_t vocab, int D, int chunk, int64_t n_chunks, const uint32_t *__restrict__ skey,
                                                                 float scale, const float *__restrict__ partial, T *__restrict__ dtable) {
   const int64_t b = (int64_t)blockIdx.x + 1;
   const int64_t at = b * chunk;
   const uint32_t key = skey[at];
   const uint32_t prev = skey[at - 1], start = b > 1 ? skey[at - chunk - 1] : 0xffffffffu;
-  if (key >= (uint32_t)V || prev != key || start == key) return;  // (start == key: an earlier border owns the row)
+  if (key >= (uint32_t)vocab || prev != key || start == key) return;  // (start == key: an earlier border owns the row)
   __shared__ int64_t end;
-  __shared__ float sum[8][32];
+  __shared__ __align__(16) float sum[8][32 * V];
   if (threadIdx.x < kWave) {  // the last chunk that begins within the row, by the chunks' first keys
     const int64_t behind = b + lower_bound_wave(skey + at, chunk, n_chunks - b, key + 1);
     if (threadIdx.x == 0) end = behind - 1;
@@ -298,27 +302,35 @@ __global__ __launch_bounds__(kBlock) void embedding_join_kernel(int64_t n, int64
   const int col = threadIdx.x & 31, sub = threadIdx.x >> 5;
   const int64_t m = end - b + 1, len = (m + 7) / 8;  // chunks b .. end, an eighth each
   const int64_t lo = b + sub * len, hi = lo + len < end + 1 ? lo + len : end + 1;
-  for (int c0 = (int)blockIdx.y * 32; c0 < D; c0 += (int)gridDim.y * 32) {
-    const int c = c0 + col;
-    float a = 0.0f;
+  for (int c0 = (int)blockIdx.y * 32 * V; c0 < D; c0 += (int)gridDim.y * 32 * V) {
+    const int c = c0 + col * V;
+    float a[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) a[v] = 0.0f;
     if (c < D) {
-      if (sub == 0) a = partial[(2 * (b - 1) + 1) * (int64_t)D + c];
+      if (sub == 0) load_vec<V>(partial + (2 * (b - 1) + 1) * (int64_t)D + c, a);
       int64_t k = lo;
       for (; k + 7 < hi; k += 8) {
-        float p[8];
+        float p[8][V];
 #pragma unroll
-        for (int u = 0; u < 8; u++) p[u] = partial[2 * (k + u) * (int64_t)D + c];
-        a += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        for (int u = 0; u < 8; u++) load_vec<V>(partial + 2 * (k + u) * (int64_t)D + c, p[u]);
+#pragma unroll
+        for (int v = 0; v < V; v++) a[v] += ((p[0][v] + p[1][v]) + (p[2][v] + p[3][v])) + ((p[4][v] + p[5][v]) + (p[6][v] + p[7][v]));
       }
-      for (; k < hi; k++) a += partial[2 * k * (int64_t)D + c];
+      for (; k < hi; k++) {
+        float p[V];
+        load_vec<V>(partial + 2 * k * (int64_t)D + c, p);
+#pragma unroll
+        for (int v = 0; v < V; v++) a[v] += p[v];
+      }
     }
-    sum[sub][col] = a;
+    store_vec<V>(&sum[sub][col * V], a);
     __syncthreads();
-    if (sub == 0 && c < D) {
+    for (int e = threadIdx.x; e < 32 * V; e += kBlock) {
       float s = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; k++) s += sum[k][col];
-      dtable[(int64_t)key * D + c] = from_f32<T>(s * scale);
+      for (int k = 0; k < 8; k++) s += sum[k][e];
+      if (c0 + e < D) dtable[(int64_t)key * D + c0 + e] = from_f32<T>(s * scale);
     }
     __syncthreads();
   }
@@ -422,16 +434,22 @@ static int bwd(int64_t n, int64_t V, int64_t D, const uint32_t *key, const int *
   const int fill_rows = (int)(65536 / rowb < 1 ? 1 : 65536 / rowb > 256 ? 256 : 65536 / rowb);
   const int64_t fill = (V + fill_rows - 1) / fill_rows, work = (n_chunks + per - 1) / per * tiles;
   if (fill + work > INT32_MAX) return DGS_ERANGE;
+  // zeros past the caches up to the last level's 256 MB (an 87 MB table: 46 us, through them 52), through them beyond (1 GB: 219 us, past 249)
+  const int keep = V * rowb > ((int64_t)256 << 20);
   const dim3 grid((unsigned)(work + fill));
   if (vec)
-    hipLaunchKernelGGL((embedding_bwd_kernel<T, true>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, (int)tiles, work, fill_rows, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
+    hipLaunchKernelGGL((embedding_bwd_kernel<T, true>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, (int)tiles, work, fill_rows, keep, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
   else
-    hipLaunchKernelGGL((embedding_bwd_kernel<T, false>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, (int)tiles, work, fill_rows, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
+    hipLaunchKernelGGL((embedding_bwd_kernel<T, false>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, (int)tiles, work, fill_rows, keep, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
   if (check_launch() != DGS_OK) return DGS_ELAUNCH;
   if (n_chunks > 1) {
     const int64_t cols = (D + 31) / 32;
-    hipLaunchKernelGGL((embedding_join_kernel<T>), dim3((unsigned)(n_chunks - 1), (unsigned)(cols < 16 ? cols : 16)), dim3(kBlock), 0, st, n, V, (int)D, chunk, n_chunks, key, scale,
-                       partial, (T *)dtable);
+    if (D % 4 == 0)
+      hipLaunchKernelGGL((embedding_join_kernel<T, 4>), dim3((unsigned)(n_chunks - 1), (unsigned)((cols + 3) / 4 < 16 ? (cols + 3) / 4 : 16)), dim3(kBlock), 0, st, n, V, (int)D, chunk,
+                         n_chunks, key, scale, partial, (T *)dtable);
+    else
+      hipLaunchKernelGGL((embedding_join_kernel<T, 1>), dim3((unsigned)(n_chunks - 1), (unsigned)(cols < 16 ? cols : 16)), dim3(kBlock), 0, st, n, V, (int)D, chunk, n_chunks, key, scale,
+                         partial, (T *)dtable);
   }
   return check_launch();
 }

@@ -348,12 +348,15 @@ __global__ __launch_bounds__(kBlock) void join_splits_kernel(int64_t count, int 
 // and LDS for a product, but there have to be enough of them: the largest whose tiles (times splits of K, where the caller can split)
 // fill three quarters of the CUs.
 enum Shape { kBig, kMid, kSmall };
+#ifndef DGS_F32_SHAPE
+#define DGS_F32_SHAPE kMid
+#endif
 struct TilePlan { Shape shape; int tiles_m, tiles_n, splits; };
 static TilePlan tile_plan(int64_t M, int64_t N, int64_t steps, int mats, bool dual, bool big, bool split) {
   TilePlan p = {kSmall, 0, 0, 1};
   const int sizes[] = {256, 128, 64};
   const int64_t cus = cu_count(), want = cus * 3 / 4;
-  for (int s = big ? kBig : kMid; s <= kSmall; s++) {
+  for (int s = big ? kBig : DGS_F32_SHAPE; s <= kSmall; s++) {
     const int64_t tm = (M + sizes[s] - 1) / sizes[s], cols = dual ? sizes[s] / 2 : sizes[s], tn = (N + cols - 1) / cols, tiles = tm * tn * mats;
     p.shape = (Shape)s;
     p.tiles_m = (int)tm;

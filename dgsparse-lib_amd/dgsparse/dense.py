@@ -9,6 +9,12 @@ from typing import Optional, Tuple
 
 import torch
 
+from . import _ops  # noqa: F401  (registers torch.ops.dgsparse_spmm.*)
+
+_op = torch.ops.dgsparse_spmm
+_embedding, _rms_norm, _add_rms_norm, _add_rms_norm_fp8 = _op.embedding.default, _op.rms_norm.default, _op.add_rms_norm.default, _op.add_rms_norm_fp8.default
+_gated_ffn, _quantize_fp8, _matmul_fp8 = _op.gated_ffn.default, _op.quantize_fp8.default, _op.matmul_fp8.default
+
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     r"""``scale * table[ids]``: the rows of ``table`` [tokens, features] named by ``ids`` (int32 or int64, any shape) -> ``[*ids.shape, features]``.
@@ -21,26 +27,25 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     order of the places (the same bits on every run), zero for rows without a place."""
     if padding_idx is not None and padding_idx < 0:
         raise ValueError('dgsparse: padding_idx must not be negative (negative ids are "no token" already)')
-    return torch.ops.dgsparse_spmm.embedding(ids, table, scale, -1 if padding_idx is None else padding_idx)
+    return _embedding(ids, table, scale, -1 if padding_idx is None else padding_idx)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     r"""``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension.  Gradients of ``x`` and ``weight``."""
-    return torch.ops.dgsparse_spmm.rms_norm(x, weight, eps)
+    return _rms_norm(x, weight, eps)
 
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     r"""``s = x + residual`` (rounded to their type: the residual of the next layer) and ``y = rms_norm(s, weight)`` in one pass over the
     rows -> ``(y, s)``.  Gradients of all three inputs; those of ``x`` and ``residual`` are one tensor."""
-    return torch.ops.dgsparse_spmm.add_rms_norm(x, residual, weight, eps)
+    return _add_rms_norm(x, residual, weight, eps)
 
 
 def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) \
         -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     r"""``add_rms_norm`` with the normed rows in 8 bits, for :func:`matmul_fp8` -> ``(q, scale, s)``: ``q`` in ``float8_e4m3fn`` and, for each
     row and block of 128 features, ``scale = max |y| / 448``; ``y`` is ``q * scale``.  For serving: it records no gradient."""
-    with torch.no_grad():
-        return torch.ops.dgsparse_spmm.add_rms_norm_fp8(x, residual, weight, eps)
+    return _add_rms_norm_fp8(x, residual, weight, eps)
 
 
 _ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
@@ -56,7 +61,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activat
     and takes no more than 1 GiB.  Both ways give results within the rounding of the other (the same bits from 65 rows on)."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f'dgsparse: activation must be one of {sorted(_ACTIVATIONS)}, not {activation!r}')
-    return torch.ops.dgsparse_spmm.gated_ffn(x, w_gate, w_up, _ACTIVATIONS[activation], -1 if recompute is None else int(not recompute))
+    return _gated_ffn(x, w_gate, w_up, _ACTIVATIONS[activation], -1 if recompute is None else int(not recompute))
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -64,8 +69,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Tensor, to
     ``block_rows`` x 128 values; ``x`` is ``q * scale``.  ``block_rows=1`` (a scale for each row: activations) or ``128`` (weights; 2-D)."""
     if block_rows not in (1, 128):
         raise ValueError(f'dgsparse: block_rows must be 1 or 128, not {block_rows}')
-    with torch.no_grad():
-        return torch.ops.dgsparse_spmm.quantize_fp8(x, block_rows)
+    return _quantize_fp8(x, block_rows)
 
 
 def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -73,5 +77,4 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     r"""``a @ b.T`` of 8-bit operands with a scale for each block of 128: ``a`` [..., K] with ``a_scale`` [..., ceil(K / 128)]
     (:func:`add_rms_norm_fp8`, ``quantize_fp8(x)``), ``b`` [N, K] with ``b_scale`` [ceil(N / 128), ceil(K / 128)] (``quantize_fp8(w, 128)``) ->
     [..., N] in ``out_dtype``.  Sums in 32 bits, one rounding.  For serving: it records no gradient."""
-    with torch.no_grad():
-        return torch.ops.dgsparse_spmm.matmul_fp8(a, a_scale, b, b_scale, out_dtype)
+    return _matmul_fp8(a, a_scale, b, b_scale, out_dtype)
