@@ -149,40 +149,35 @@ __global__ __launch_bounds__(512) void gated_few_kernel(const char *__restrict__
   const char *px[FM];
 #pragma unroll
   for (int i = 0; i < FM; i++) px[i] = x + (int64_t)(16 * i + r < M ? 16 * i + r : M - 1) * ldx + (lane >> 4) * 16;
-  f32x4 ag[FM], au[FM];
+  f32x4 acc[FM][2];
 #pragma unroll
-  for (int i = 0; i < FM; i++) ag[i] = au[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < FM; i++) acc[i][0] = acc[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const dgs_u4 zero = {0u, 0u, 0u, 0u};
   constexpr int U = FM == 1 ? 4 : 2;  // 128-byte steps in flight
   for (int64_t k0 = wave * 128; k0 < kbytes; k0 += kW * 128 * U) {
-    Slice g[U][2], u[U][2], a[U][2][FM];
+    Slice w[U][2][2], a[U][2][FM];  // (the rows of Wg and of Wu)
 #pragma unroll
     for (int s = 0; s < U; s++)
 #pragma unroll
       for (int kk = 0; kk < 2; kk++) {
         const int64_t k = k0 + (int64_t)s * kW * 128 + kk * 64;
         const bool on = k + (lane >> 4) * 16 < kbytes;
-        g[s][kk].u = on ? __builtin_nontemporal_load((const dgs_u4 *)(pg + k)) : zero;
-        u[s][kk].u = on ? __builtin_nontemporal_load((const dgs_u4 *)(pu + k)) : zero;
+        w[s][kk][0].u = on ? __builtin_nontemporal_load((const dgs_u4 *)(pg + k)) : zero;
+        w[s][kk][1].u = on ? __builtin_nontemporal_load((const dgs_u4 *)(pu + k)) : zero;
 #pragma unroll
         for (int i = 0; i < FM; i++) a[s][kk][i].u = on ? *(const dgs_u4 *)(px[i] + k) : zero;
       }
 #pragma unroll
     for (int s = 0; s < U; s++)
 #pragma unroll
-      for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-        for (int i = 0; i < FM; i++) {
-          Mma<T>::step(ag[i], g[s][kk], a[s][kk][i]);
-          Mma<T>::step(au[i], u[s][kk], a[s][kk][i]);
-        }
+      for (int kk = 0; kk < 2; kk++) multiply<T>(a[s][kk], w[s][kk], acc);
   }
 #pragma unroll
   for (int i = 0; i < FM; i++)
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      sum[wave][0][16 * i + r][4 * (lane >> 4) + k] = ag[i][k];
-      sum[wave][1][16 * i + r][4 * (lane >> 4) + k] = au[i][k];
+      sum[wave][0][16 * i + r][4 * (lane >> 4) + k] = acc[i][0][k];
+      sum[wave][1][16 * i + r][4 * (lane >> 4) + k] = acc[i][1][k];
     }
   __syncthreads();
   for (int e = threadIdx.x; e < 256 * FM; e += 512) {

@@ -15,6 +15,8 @@
 // Sums are held in 32 bits throughout; K is walked in order, so a result depends on the tile shape and the number of splits alone, and
 // these on the sizes alone.
 #pragma once
+#include <type_traits>
+
 #include "dense_common.h"
 
 namespace dgs {
@@ -42,19 +44,24 @@ union Slice {
   float f[4];
   s16x4 s[2];
 };
-template <typename T> struct Mma;
-template <> struct Mma<bf16> {
-  static __device__ __forceinline__ void step(f32x4 &c, const Slice &b, const Slice &a) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.b, a.b, c, 0, 0, 0); }
-};
-template <> struct Mma<f16> {
-  static __device__ __forceinline__ void step(f32x4 &c, const Slice &b, const Slice &a) { c = __builtin_amdgcn_mfma_f32_16x16x32_f16(b.h, a.h, c, 0, 0, 0); }
-};
-template <> struct Mma<float> {  // lane group g holds k = 4 g .. 4 g + 3: the j-th of four instructions takes the j-th of them
-  static __device__ __forceinline__ void step(f32x4 &c, const Slice &b, const Slice &a) {
+// acc[i][j] += a[i] b[j] over the slice.  32 bits: lane group g holds k = 4 g .. 4 g + 3, and the q-th of four instructions takes the q-th
+// of them; the four go round all sums, so that none waits for the one before.
+template <typename T, int FM, int FN>
+__device__ __forceinline__ void multiply(const Slice (&a)[FM], const Slice (&b)[FN], f32x4 (&acc)[FM][FN]) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(b.f[j], a.f[j], c, 0, 0, 0);
-  }
-};
+  for (int q = 0; q < (sizeof(T) == 4 ? 4 : 1); q++)
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+      for (int j = 0; j < FN; j++) {
+        if constexpr (sizeof(T) == 4)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j].f[q], a[i].f[q], acc[i][j], 0, 0, 0);
+        else if constexpr (std::is_same<T, f16>::value)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[j].h, a[i].h, acc[i][j], 0, 0, 0);
+        else
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j].b, a[i].b, acc[i][j], 0, 0, 0);
+      }
+}
 
 // ---- one operand's tile in LDS: R rows (of M or N) x 128 bytes of K, R * 128 bytes -------------------------------------------------
 template <typename T, int R, bool KO>
@@ -226,10 +233,7 @@ struct Gemm {
       for (int j = 0; j < FN; j++) TB::read(lb, b_row(wn, j), kk, lane, b[j]);
 #pragma unroll
       for (int i = 0; i < FM; i++) TA::read(la, wm * (BM / WM) + 16 * i, kk, lane, a[i]);
-#pragma unroll
-      for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++) Mma<T>::step(acc[i][j], b[j], a[i]);
+      multiply<T>(a, b, acc);
     }
   }
 };
