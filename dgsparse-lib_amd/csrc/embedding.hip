@@ -15,7 +15,7 @@
 
 namespace dgs {
 
-constexpr int kSortSmall = 4096;   // positions up to here: one launch that counts ranks
+constexpr int kSortSmall = 8192;   // positions up to here: one launch that counts ranks (n^2 comparisons; at 8192 either sort makes 53 us with an 87 MB gradient behind it, at 4000 this one 42)
 constexpr int kSortWaves = 8;      // waves of a radix-sort workgroup
 constexpr int kSortBits = 9;       // at most this many bits a pass (512 bins)
 constexpr int kSortBlocks = 256;   // at most this many workgroups a pass (each reads all the others' counts)
@@ -54,37 +54,44 @@ __global__ __launch_bounds__(kBlock) void embedding_fwd_kernel(int64_t n, int64_
 }
 
 // ---- sorting ---------------------------------------------------------------------------------------------------------------
-// Few positions: the place of (key, p) in the sorted list is the number of pairs in front of it.  A workgroup ranks 32 positions, 8
-// threads each an eighth of the list out of LDS; no pass waits for another.
+// Few positions: the place of (key, p) in the sorted list is the number of pairs in front of it.  A workgroup ranks 16 positions, 16
+// threads each a sixteenth of the list out of LDS, four keys a read; no pass waits for another.
 template <typename I>
 __global__ __launch_bounds__(kBlock) void embedding_rank_kernel(int n, int64_t V, int64_t pad, const I *__restrict__ ids,
                                                                 uint32_t *__restrict__ skey, int *__restrict__ spos) {
-  __shared__ uint32_t key[kSortSmall];
-  __shared__ int part[8][32];
-  for (int p = threadIdx.x; p < n; p += kBlock) key[p] = token_key(ids[p], V, pad);
+  __shared__ __align__(16) uint32_t key[kSortSmall];
+  __shared__ int part[16][16];
+  const int n4 = (n + 3) / 4;
+  for (int p = threadIdx.x; p < 4 * n4; p += kBlock) key[p] = p < n ? token_key(ids[p], V, pad) : 0xffffffffu;  // (behind the list: behind every pair)
   __syncthreads();
-  const int mine = threadIdx.x & 31, sub = threadIdx.x >> 5;
-  const int p = blockIdx.x * 32 + mine;
-  int before = 0;
+  const int mine = threadIdx.x & 15, sub = threadIdx.x >> 4;
+  const int p = blockIdx.x * 16 + mine;
   const uint32_t k = p < n ? key[p] : 0u;
-  const int len = (n + 7) / 8, lo = sub * len, hi = lo + len < n ? lo + len : n;
-  for (int o = lo; o < hi; o++) before += key[o] < k || (key[o] == k && o < p);
+  const int len = (n4 + 15) / 16, lo = sub * len, hi = lo + len < n4 ? lo + len : n4;
+  int before = 0;
+#pragma unroll 4
+  for (int o = lo; o < hi; o++) {
+    const dgs_u4 v = *reinterpret_cast<const dgs_u4 *>(&key[4 * o]);
+#pragma unroll
+    for (int j = 0; j < 4; j++) before += (v[j] < k) | ((v[j] == k) & (4 * o + j < p));
+  }
   part[sub][mine] = before;
   __syncthreads();
   if (sub == 0 && p < n) {
     int at = 0;
 #pragma unroll
-    for (int s = 0; s < 8; s++) at += part[s][mine];
+    for (int s = 0; s < 16; s++) at += part[s][mine];
     skey[at] = k;
     spos[at] = p;
   }
 }
 
-// Many positions: a stable radix sort from the low digit, two launches a pass (counts, then placement), `tile` positions a workgroup.
+// Many positions: a stable radix sort from the low digit, `tile` positions a workgroup, two launches a pass: counts, then placement.  (Counting
+// the next digit while placing saves a launch and loses more to the adds that meet on a frequent token's counter: 77 -> 86 us for
+// 100003 positions of a Zipf law with the gradient behind it.)
 template <typename I>
 __global__ __launch_bounds__(kSortWaves *kWave) void embedding_count_kernel(int64_t n, int64_t V, int64_t pad, int tile, int shift, int bits,
-                                                                            const I *__restrict__ ids, const uint32_t *__restrict__ kin,
-                                                                            int *__restrict__ hist) {
+                                                                            const I *__restrict__ ids, const uint32_t *__restrict__ kin, int *__restrict__ hist) {
   __shared__ int cnt[1 << kSortBits];
   const int bins = 1 << bits;
   for (int b = threadIdx.x; b < bins; b += blockDim.x) cnt[b] = 0;
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(kSortWaves *kWave) void embedding_place_kernel(int6
   // this thread's digit: positions with it in all workgroups, and in those in front of this one
   int all = 0, front = 0;
   if (t < bins) {
-#pragma unroll 16
+#pragma unroll 32
     for (int b = 0; b < (int)gridDim.x; b++) {  // (independent reads out of L2: as many as registers take are in flight)
       const int h = hist[(int64_t)b * bins + t];
       all += h;
@@ -358,9 +365,8 @@ static SortPlan sort_plan(int64_t n, int64_t V) {
   const int kb = key_bits(V);
   p.passes = (kb + kSortBits - 1) / kSortBits;
   p.bits = (kb + p.passes - 1) / p.passes;
-  const int64_t least = kSortWaves * kWave;  // 64 positions a wave
-  int64_t tile = (n + kSortBlocks - 1) / kSortBlocks;
-  tile = tile < 2 * least ? 2 * least : (tile + least - 1) / least * least;
+  int64_t tile = 2 * kSortWaves * kWave;  // 128 positions a wave at least
+  while ((n + tile - 1) / tile > kSortBlocks) tile *= 2;
   p.tile = (int)tile;
   p.blocks = (n + tile - 1) / tile;
   return p;
@@ -400,17 +406,17 @@ static int sort_ids(int64_t n, int64_t V, int64_t pad, const I *ids, char *ws, c
   if (n <= kSortSmall) {
     *key = (uint32_t *)(ws + L.key[0]);
     *pos = (int *)(ws + L.pos[0]);
-    hipLaunchKernelGGL((embedding_rank_kernel<I>), dim3((unsigned)((n + 31) / 32)), dim3(kBlock), 0, st, (int)n, V, pad, ids, *key, *pos);
+    hipLaunchKernelGGL((embedding_rank_kernel<I>), dim3((unsigned)((n + 15) / 16)), dim3(kBlock), 0, st, (int)n, V, pad, ids, *key, *pos);
     return check_launch();
   }
   const SortPlan p = sort_plan(n, V);
   int *hist = (int *)(ws + L.hist);
+  const dim3 grid((unsigned)p.blocks), block(kSortWaves * kWave);
   const uint32_t *kin = nullptr;
   const int *pin = nullptr;
   for (int i = 0; i < p.passes; i++) {
     uint32_t *kout = (uint32_t *)(ws + L.key[i & 1]);
     int *pout = (int *)(ws + L.pos[i & 1]);
-    const dim3 grid((unsigned)p.blocks), block(kSortWaves * kWave);
     hipLaunchKernelGGL((embedding_count_kernel<I>), grid, block, 0, st, n, V, pad, p.tile, i * p.bits, p.bits, ids, kin, hist);
     hipLaunchKernelGGL((embedding_place_kernel<I>), grid, block, 0, st, n, V, pad, p.tile, i * p.bits, p.bits, ids, kin, pin, hist, kout, pout);
     if (check_launch() != DGS_OK) return DGS_ELAUNCH;

@@ -77,7 +77,7 @@ def check_embedding(ids, table, scale=1.0, pad=None, seed=0, dout=None):
 
 @pytest.mark.parametrize('t', TYPES, ids=ids_of)
 @pytest.mark.parametrize('n,V,D', [(1, 1, 1), (1, 7, 8), (2, 3, 5), (33, 50, 130), (64, 3, 1000), (31, 33, 4096), (257, 100, 24), (4096, 300, 16),
-                                   (4097, 300, 16), (5000, 97, 40), (20000, 70000, 8), (9000, 1 << 19, 3), (3000, 129, 2056)])
+                                   (4097, 300, 16), (8192, 500, 8), (8193, 500, 8), (10000, 97, 40), (20000, 70000, 8), (9000, 1 << 19, 3), (9000, (1 << 20) + 7, 2), (3000, 129, 2056)])
 def test_embedding_matches_64_bits(n, V, D, t):
     g = torch.Generator(device='cuda').manual_seed(n)
     ids = torch.randint(0, V, (n,), generator=g, device='cuda')
@@ -92,10 +92,10 @@ def test_embedding_no_token_beyond_the_table_and_padding(t):
     assert dtable[2].eq(0).all() and dtable[1].eq(0).all() and dtable[0].ne(0).any()
     # not one token at all
     check_embedding(torch.full((70,), -1, device='cuda'), rand(5, 12, t=t, seed=3))
-    check_embedding(torch.full((5000,), 5, device='cuda', dtype=torch.int32), rand(5, 12, t=t, seed=3))
+    check_embedding(torch.full((9000,), 5, device='cuda', dtype=torch.int32), rand(5, 12, t=t, seed=3))
 
 
-@pytest.mark.parametrize('n', [65, 3000, 6000])
+@pytest.mark.parametrize('n', [65, 3000, 20000])
 def test_embedding_one_token_at_every_place(n):
     """The row's sum crosses every chunk's border; its neighbours have none, or one at the list's ends."""
     ids = torch.full((n,), 3, device='cuda')
