@@ -62,15 +62,14 @@ __global__ __launch_bounds__(64 * WM *WN) void fp8_kernel(const GemmArgs g, cons
   for (int i = 0; i < G::FM; i++)
 #pragma unroll
     for (int j = 0; j < G::FN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const int64_t nlast = (g.N - 1) / 128, nb = (n0 + wn * (BN / WN)) / 128;
-  const float *sb = sc.b + (nb < nlast ? nb : nlast) * sc.blocks;
-  // The scales of a for kWindow steps at a time, by way of LDS: the loads take them in rows of kWindow neighbours (a lane's own loads of them
-  // would touch 16 lines a wave and 16 rows: 305 us instead of 205 + for 4095 x 11000 x 4096).  Two windows: the next one is loaded in the
-  // first step of this one.  Rows behind the matrix are behind the descriptor: 0.
+  // The scales for kWindow steps at a time, by way of LDS: the loads take them in rows of kWindow neighbours (a lane's own loads of them
+  // would touch 16 lines for each 16 rows: 305 us instead of 221 for 4095 x 11000 x 4096).  Two windows: the next one is loaded in the first
+  // step of this one.  Rows behind the matrix are behind the descriptor: 0.
   constexpr int kScaleLoads = BM * kWindow / G::kThreads;
-  __shared__ __align__(16) float scales[2][BM * kWindow];
-  const int64_t scale_bytes = (g.M - m0) * sc.blocks * 4;
+  __shared__ __align__(16) float scales[2][BM * kWindow + 64];  // (behind a's: b's, a row of kWindow for each 128 columns)
+  const int64_t scale_bytes = (g.M - m0) * sc.blocks * 4, nb = n0 / 128, b_bytes = ((g.N + 127) / 128 - nb) * sc.blocks * 4;
   const auto sa = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(sc.a + m0 * sc.blocks), 0, scale_bytes < kRange ? (int)scale_bytes : kRange, 0x00027000);
+  const auto sb = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(sc.b + nb * sc.blocks), 0, b_bytes < kRange ? (int)b_bytes : kRange, 0x00027000);
   auto load_window = [&](int w) {  // steps s0 + w kWindow ...
     const int s = s0 + w * kWindow + (int)threadIdx.x % kWindow;
 #pragma unroll
@@ -78,13 +77,22 @@ __global__ __launch_bounds__(64 * WM *WN) void fp8_kernel(const GemmArgs g, cons
       const int row = (q * G::kThreads + (int)threadIdx.x) / kWindow;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(sa, (lds_void *)(lds_char *)(&scales[w & 1][(q * G::kWaves + wave) * 64]), 4, s < s1 ? (row * (int)sc.blocks + s) * 4 : (int)kNowhere, 0, 0, 0);
     }
+    if (wave == 0) {
+      const int row = lane / kWindow;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (lds_void *)(lds_char *)(&scales[w & 1][BM * kWindow]), 4, s < s1 && row < (BN + 127) / 128 ? (row * (int)sc.blocks + s) * 4 : (int)kNowhere, 0, 0, 0);
+    }
   };
-  float f[G::FM];
-  auto take_scales = [&](int s) {
-    const float t = sb[s];
-    const float *p = &scales[((s - s0) / kWindow) & 1][(wm * (BM / WM) + (lane & 15)) * kWindow + (s - s0) % kWindow];
+  // a step's scales are read from LDS a step ahead
+  float f[G::FM], ahead[G::FM], ahead_b = 0.0f;
+  auto fetch_scales = [&](int s) {
+    const float *p = scales[((s - s0) / kWindow) & 1] + (s - s0) % kWindow;
+    ahead_b = p[(BM + ((n0 + wn * (BN / WN)) / 128 - (int)nb)) * kWindow];
 #pragma unroll
-    for (int i = 0; i < G::FM; i++) f[i] = p[16 * i * kWindow] * t;
+    for (int i = 0; i < G::FM; i++) ahead[i] = p[(wm * (BM / WM) + (lane & 15) + 16 * i) * kWindow];
+  };
+  auto take_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < G::FM; i++) f[i] = ahead[i] * ahead_b;
   };
   auto compute = [&](const char *la, const char *lb) {
     Slice8 b[G::FN];
@@ -125,19 +133,24 @@ __global__ __launch_bounds__(64 * WM *WN) void fp8_kernel(const GemmArgs g, cons
     load_window(0);
     G::load(l, g, m0, n0, s0, steps, 0, ldsA0, ldsB0);
     loads_done();
+    fetch_scales(s0);
     int s = s0;
     for (; s + 1 < s1; s += 2) {
-      take_scales(s);
+      take_scales();
+      fetch_scales(s + 1);  // (an odd step of a window: there)
       if ((s - s0) % kWindow == 0 && s + kWindow < s1) load_window((s - s0) / kWindow + 1);
       G::load(l, g, m0, n0, s + 1, steps, 0, ldsA1, ldsB1);
       compute(ldsA0, ldsB0);
       loads_done();
-      take_scales(s + 1);
-      if (s + 2 < s1) G::load(l, g, m0, n0, s + 2, steps, 0, ldsA0, ldsB0);
+      take_scales();
+      if (s + 2 < s1) {
+        fetch_scales(s + 2);  // (a new window's first step: loaded since this window's first step)
+        G::load(l, g, m0, n0, s + 2, steps, 0, ldsA0, ldsB0);
+      }
       compute(ldsA1, ldsB1);
       loads_done();
     }
-    if (s < s1) take_scales(s);
+    take_scales();
     if (s < s1) compute(ldsA0, ldsB0);
   }
 #pragma unroll
@@ -348,7 +361,7 @@ static int matmul8(int64_t M, int64_t N, int64_t K, const void *a, int64_t lda, 
   bool done = false;
   if constexpr (sizeof(T) == 2) {
     if (p.shape == kBig) {
-      hipLaunchKernelGGL((fp8_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, g, sc, out, partial);
+      hipLaunchKernelGGL((fp8_kernel<T, 256, 256, 4, 2>), grid, dim3(512), 0, st, g, sc, out, partial);
       done = true;
     }
   }
