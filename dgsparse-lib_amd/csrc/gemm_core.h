@@ -67,12 +67,20 @@ __device__ __forceinline__ void multiply(const Slice (&a)[FM], const Slice (&b)[
 // nearest from what is left.  A product of two such values is six products of their parts, the ones below 2^-26 of it left out: as close
 // as a product rounded to 32 bits, on matrix instructions that take the six (96 cycles for 16 x 16 x 32) in less than half the time of the
 // 32-bit ones (256).  The parts' products are exact, their sums held in 32 bits.  What differs: an infinity becomes a NaN (inf - inf).
+//
+// What is left of a value is one instruction, the dot product of its pair's parts with (-1, 0) or (0, -1) added to it: exact, like the
+// subtraction it stands for, without the part widened to 32 bits first (7 instructions a pair for the three parts, not 11).  The constants
+// are kept in registers: as inline constants these instructions take them for both halves.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 struct Three {
   bf16x8 p[3];
 };
-__device__ __forceinline__ void split3(const Slice &x0, const Slice &x1, Three &t) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
+struct Minus {  // (-1, 0) and (0, -1) in bf16
+  uint32_t lo = 0x0000bf80u, hi = 0xbf800000u;
+  __device__ __forceinline__ Minus() { asm volatile("" : "+s"(lo), "+s"(hi)); }
+};
+__device__ __forceinline__ void split3(const Slice &x0, const Slice &x1, const Minus &minus, Three &t) {
   union { bf16x8 v; uint32_t u[4]; } p[3];
 #pragma unroll
   for (int k = 0; k < 4; k++) {
@@ -80,11 +88,11 @@ __device__ __forceinline__ void split3(const Slice &x0, const Slice &x1, Three &
     f32x2 r = {x[0], x[1]};
 #pragma unroll
     for (int q = 0; q < 3; q++) {
-      const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
-      p[q].u[k] = h;
+      const bf16x2 h = __builtin_convertvector(r, bf16x2);
+      p[q].u[k] = __builtin_bit_cast(uint32_t, h);
       if (q < 2) {
-        r[0] -= __builtin_bit_cast(float, h << 16);
-        r[1] -= __builtin_bit_cast(float, h & 0xffff0000u);
+        r[0] = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, minus.lo), r[0], false);
+        r[1] = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, minus.hi), r[1], false);
       }
     }
   }
@@ -256,13 +264,14 @@ struct Gemm {
   static __device__ __forceinline__ void compute(const char *la, const char *lb, int wm, int wn, int lane, f32x4 (&acc)[FM][FN]) {
     if constexpr (sizeof(T) == 4) {
       // (a lane's 8 values of K: 4 of each half of the step, the same in both operands)
+      const Minus minus;
       Three b[FN];
 #pragma unroll
       for (int j = 0; j < FN; j++) {
         Slice x0, x1;
         TB::read(lb, b_row(wn, j), 0, lane, x0);
         TB::read(lb, b_row(wn, j), 1, lane, x1);
-        split3(x0, x1, b[j]);
+        split3(x0, x1, minus, b[j]);
       }
 #pragma unroll
       for (int i = 0; i < FM; i++) {
@@ -270,7 +279,7 @@ struct Gemm {
         Three a;
         TA::read(la, wm * (BM / WM) + 16 * i, 0, lane, x0);
         TA::read(la, wm * (BM / WM) + 16 * i, 1, lane, x1);
-        split3(x0, x1, a);
+        split3(x0, x1, minus, a);
         constexpr int pa[6] = {0, 2, 1, 0, 1, 0}, pb[6] = {2, 0, 1, 1, 0, 0};  // the small ones first
 #pragma unroll
         for (int q = 0; q < 6; q++)
