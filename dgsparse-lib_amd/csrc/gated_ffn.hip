@@ -290,10 +290,11 @@ template <typename T, int ACT, bool BWD>
 static int launch_gated(int64_t rows, int64_t D, int64_t F, const Operands<T> &op, const GatedOut &out, hipStream_t st) {
   constexpr int kK = kStepBytes / (int)sizeof(T);
   const int64_t cols = BWD ? out.ldo : F;
-  const TilePlan p = tile_plan(rows, cols, (D + kK - 1) / kK, 1, true, sizeof(T) == 2, false);
+  constexpr bool kWide = sizeof(T) == 2 || !BWD;  // (32 bits: forward 417 -> 369 us of 169343 x 128 x 512, backward 488 -> 523)
+  const TilePlan p = tile_plan(rows, cols, (D + kK - 1) / kK, 1, true, kWide, false);
   GemmArgs g = {{op.x, nullptr}, {op.wg, op.wu}, op.ldx * (int64_t)sizeof(T), op.ldw * (int64_t)sizeof(T), rows, F, D, p.tiles_m, p.tiles_n, 1};
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n));
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (kWide) {
     if (p.shape == kBig) {
       hipLaunchKernelGGL((gated_kernel<T, 256, 256, 2, 4, ACT, BWD>), grid, dim3(512), 0, st, g, out);
       return check_launch();

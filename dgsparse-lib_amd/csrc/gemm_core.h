@@ -412,19 +412,20 @@ __global__ __launch_bounds__(kBlock) void join_splits_kernel(int64_t count, int 
 
 // ---- which tile, how many splits ------------------------------------------------------------------------------------------
 // kBig: 256 x 256, 8 waves, a workgroup a CU; kMid: 128 x 128, 4 waves, 2 a CU; kSmall: 64 x 64, 4 waves.  A larger tile reads less from L2
-// and LDS for a product, but there have to be enough of them: the largest whose tiles (times splits of K, where the caller can split)
-// fill three quarters of the CUs.
+// and LDS for a product, but there have to be enough of them, and they must not lie half beside the matrix: the largest whose tiles (times
+// splits of K, where the caller can split) fill three quarters of the CUs and cover at most a quarter more than the next smaller ones.
 enum Shape { kBig, kMid, kSmall };
-#ifndef DGS_F32_SHAPE
-#define DGS_F32_SHAPE kMid
-#endif
 struct TilePlan { Shape shape; int tiles_m, tiles_n, splits; };
 static TilePlan tile_plan(int64_t M, int64_t N, int64_t steps, int mats, bool dual, bool big, bool split) {
   TilePlan p = {kSmall, 0, 0, 1};
   const int sizes[] = {256, 128, 64};
   const int64_t cus = cu_count(), want = cus * 3 / 4;
-  for (int s = big ? kBig : DGS_F32_SHAPE; s <= kSmall; s++) {
+  for (int s = big ? kBig : kMid; s <= kSmall; s++) {
     const int64_t tm = (M + sizes[s] - 1) / sizes[s], cols = dual ? sizes[s] / 2 : sizes[s], tn = (N + cols - 1) / cols, tiles = tm * tn * mats;
+    if (s < kSmall) {
+      const int64_t half = sizes[s] / 2, least = ((M + half - 1) / half) * ((N + cols / 2 - 1) / (cols / 2));  // in quarters of this tile
+      if (4 * tm * tn > least + least / 4) continue;
+    }
     p.shape = (Shape)s;
     p.tiles_m = (int)tm;
     p.tiles_n = (int)tn;
