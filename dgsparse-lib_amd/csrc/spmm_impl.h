@@ -674,7 +674,9 @@ __device__ __forceinline__ void acc_commit(float *__restrict__ C, int *__restric
       // (around: ids below vc.lo are the slots that precede, ids from vc.lo + vc.n on the slots that follow, shifted by vc.n)
       const int es = (around & (ei[v] >= aa.vc.lo)) ? ei[v] - aa.vc.n : ei[v];
       const int en = ei[v] >= 0 ? es + aa.col_off : -1;
-      const bool won_virt = around & ((unsigned)(ei[v] - aa.vc.lo) < (unsigned)aa.vc.n);
+      // (ei < 0: nothing improved on the identity, the virtual entry included - a NaN that ended the old pair's own chain does not, and
+      // neither did anything behind it: the old arg stands)
+      const bool won_virt = around & (((unsigned)(ei[v] - aa.vc.lo) < (unsigned)aa.vc.n) | (ei[v] < 0));
       const float a = first ? acc[v] : old[v], b = first ? old[v] : acc[v];  // a comes first in the row
       const int ea = first ? en : eo[v], eb = first ? eo[v] : en;
       const bool old_empty = (eo[v] < 0) & (old[v] != reduce_init<DGS_MIN>());

@@ -85,7 +85,7 @@ def _f(a):
     return a, a.ctypes.data_as(_f32p)
 
 
-def spmm(reduce, rowptr, col, val, B, K=None, fma=False, threads=1):
+def spmm(reduce, rowptr, col, val, B, K=None, fma=False, threads=None):  # (threads: all cores; the bits are the same for any number)
     """Algorithm-0 SpMM.  Returns (C[M,N] f32, E[M,N] i32)."""
     op = REDUCE[reduce] if isinstance(reduce, str) else int(reduce)
     rowptr, prp = _i(rowptr)
@@ -97,7 +97,7 @@ def spmm(reduce, rowptr, col, val, B, K=None, fma=False, threads=1):
     C = np.empty((M, N), np.float32)
     E = np.empty((M, N), np.int32)
     rc = lib().orc_spmm_csr_f32(op, int(fma), M, K, N, col.shape[0], prp, pc, pv, pb,
-                                C.ctypes.data_as(_f32p), E.ctypes.data_as(_i32p), int(threads))
+                                C.ctypes.data_as(_f32p), E.ctypes.data_as(_i32p), int(threads or max_threads()))
     assert rc == 0
     return C, E
 
@@ -161,7 +161,7 @@ def spmm_mask_f64(colptr, row, tval, G, E, absval=False):
     return out
 
 
-def sddmm(rowptr, col, D1, D2, reduce='sum', fma=False, threads=1):
+def sddmm(rowptr, col, D1, D2, reduce="sum", fma=False, threads=None):
     op = REDUCE[reduce] if isinstance(reduce, str) else int(reduce)
     rowptr, p0 = _i(rowptr)
     col, p1 = _i(col)
@@ -169,7 +169,7 @@ def sddmm(rowptr, col, D1, D2, reduce='sum', fma=False, threads=1):
     D2, p3 = _f(D2)
     out = np.empty(col.shape[0], np.float32)
     rc = lib().orc_sddmm_csr_f32(op, int(fma), rowptr.shape[0] - 1, D1.shape[1], col.shape[0], p0, p1,
-                                 p2, p3, out.ctypes.data_as(_f32p), int(threads))
+                                 p2, p3, out.ctypes.data_as(_f32p), int(threads or max_threads()))
     assert rc == 0
     return out
 

@@ -124,6 +124,10 @@ int orc_spmm_csr_f32(int reduce_op, int fma, int64_t M, int64_t K, int64_t N, in
  */
 int orc_spmm_csr_mask_f32(int fma, int64_t Mout, int64_t N, const int32_t *ptr, const int32_t *idx,
                           const float *val, const float *G, const int32_t *E, float *out) {
+  /* (every element is a chain of its own: the elements go round the cores, their order and bits do not change) */
+#ifdef _OPENMP
+#pragma omp parallel for collapse(2) schedule(dynamic, 64)
+#endif
   for (int64_t j = 0; j < Mout; j++) {
     for (int64_t f = 0; f < N; f++) {
       float res = 0.0f;
@@ -231,6 +235,9 @@ int orc_max_threads(void) {
  */
 int orc_spmm_sum_f64(int mean, int absval, int64_t M, int64_t N, const int32_t *rowptr, const int32_t *col,
                      const float *val, const float *B, double *C) {
+#ifdef _OPENMP
+#pragma omp parallel for schedule(dynamic, 64)
+#endif
   for (int64_t r = 0; r < M; r++) {
     const int64_t s = rowptr[r], e = rowptr[r + 1];
     for (int64_t f = 0; f < N; f++) {
@@ -285,6 +292,9 @@ int orc_gspmm_csr_f32(int reduce_op, int compute_op, int64_t M, int64_t N, const
  * entries that pass the mask (condition scale). */
 int orc_spmm_mask_f64(int absval, int64_t Mout, int64_t N, const int32_t *ptr, const int32_t *idx, const float *val,
                       const float *G, const int32_t *E, double *out) {
+#ifdef _OPENMP
+#pragma omp parallel for collapse(2) schedule(dynamic, 64)
+#endif
   for (int64_t j = 0; j < Mout; j++)
     for (int64_t f = 0; f < N; f++) {
       double res = 0.0;
