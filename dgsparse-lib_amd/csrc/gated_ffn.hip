@@ -46,6 +46,25 @@ __device__ __forceinline__ float act(float g, float &d) {
   }
 }
 
+// the product of a tile, with its LDS: 16-bit operands straight to LDS, 32-bit ones split on the way
+template <typename T, int BM, int BN, int WM, int WN, bool A_KO, bool B_KO, int PAIR>
+struct Core {
+  using G = Gemm<T, BM, BN, WM, WN, A_KO, B_KO, PAIR>;
+  static __device__ __forceinline__ void run(const GemmArgs &g, int m0, int n0, int s0, int s1, int steps, int z, int wm, int wn, int lane, f32x4 (&acc)[G::FM][G::FN]) {
+    DGS_GEMM_LDS(G)
+    gemm_loop<G>(g, m0, n0, s0, s1, steps, z, ldsA0, ldsB0, ldsA1, ldsB1, wm, wn, lane, acc);
+  }
+};
+template <int BM, int BN, int WM, int WN, bool A_KO, bool B_KO, int PAIR>
+struct Core<float, BM, BN, WM, WN, A_KO, B_KO, PAIR> {
+  using G = Gemm3<BM, BN, WM, WN, A_KO, B_KO, PAIR>;
+  static __device__ __forceinline__ void run(const GemmArgs &g, int m0, int n0, int s0, int s1, int steps, int z, int wm, int wn, int lane, f32x4 (&acc)[G::FM][G::FN]) {
+    __shared__ __align__(16) char lds[G::PA::kBytes + G::PB::kBytes];
+    G::run(g, m0, n0, s0, s1, steps, z, lds, wm, wn, lane, acc);
+  }
+};
+template <typename T> constexpr int kStepK = kStepBytes / (int)sizeof(T);  // K values a step
+
 struct GatedOut {
   const void *dh;   // backward: [M, F], contiguous
   float *pre;       // forward: where the two products are kept, [2][M, F], or null
@@ -82,16 +101,17 @@ __device__ __forceinline__ void gated_store(const GatedOut &o, int64_t M, int64_
   }
 }
 
+// (32 bits: registers for three workgroups on a CU, forward 388 -> 338 us, backward 477 -> 430 of 169343 x 128 x 512; the plain products, which
+// read K-outer tiles, would spill at that: 329 -> 410)
 template <typename T, int BM, int BN, int WM, int WN, int ACT, bool BWD>
-__global__ __launch_bounds__(64 * WM *WN) void gated_kernel(const GemmArgs g, const GatedOut o) {
-  using G = Gemm<T, BM, BN, WM, WN, false, false, kDual>;
-  DGS_GEMM_LDS(G)
+__global__ __launch_bounds__(64 * WM *WN, sizeof(T) == 4 ? 3 : 1) void gated_kernel(const GemmArgs g, const GatedOut o) {
+  using G = typename Core<T, BM, BN, WM, WN, false, false, kDual>::G;
   const Where at = where_of(g.tiles_m, g.tiles_n);
   const int m0 = at.m * BM, n0 = at.n * G::kCols;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, wm = wave / WN, wn = wave % WN;
-  const int steps = (int)((g.K + G::TA::kK - 1) / G::TA::kK);
+  const int steps = (int)((g.K + kStepK<T> - 1) / kStepK<T>);
   f32x4 acc[G::FM][G::FN];
-  gemm_loop<G>(g, m0, n0, 0, steps, steps, 0, ldsA0, ldsB0, ldsA1, ldsB1, wm, wn, lane, acc);
+  Core<T, BM, BN, WM, WN, false, false, kDual>::run(g, m0, n0, 0, steps, steps, 0, wm, wn, lane, acc);
   const bool vec = o.ldo % 4 == 0;
   const int64_t end = BWD ? o.ldo : o.F;
 #pragma unroll
@@ -204,17 +224,16 @@ struct PlainOut {
   float *partial;
 };
 template <typename T, int BM, int BN, int WM, int WN, bool A_KO, bool B_KO, int PAIR>
-__global__ __launch_bounds__(64 * WM *WN) void product_kernel(const GemmArgs g, const PlainOut o) {
-  using G = Gemm<T, BM, BN, WM, WN, A_KO, B_KO, PAIR>;
-  DGS_GEMM_LDS(G)
+__global__ __launch_bounds__(64 * WM *WN, sizeof(T) == 4 ? 2 : 1) void product_kernel(const GemmArgs g, const PlainOut o) {
+  using G = typename Core<T, BM, BN, WM, WN, A_KO, B_KO, PAIR>::G;
   const Where at = where_of(g.tiles_m, g.tiles_n);
   const int z = PAIR == kTwo ? at.z % 2 : 0, split = PAIR == kTwo ? at.z / 2 : at.z;
   const int m0 = at.m * BM, n0 = at.n * BN;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, wm = wave / WN, wn = wave % WN;
-  const int steps = (int)((g.K + G::TA::kK - 1) / G::TA::kK), all = PAIR == kSum ? 2 * steps : steps;
+  const int steps = (int)((g.K + kStepK<T> - 1) / kStepK<T>), all = PAIR == kSum ? 2 * steps : steps;
   const int per = (all + g.splits - 1) / g.splits, s0 = split * per, s1 = s0 + per < all ? s0 + per : all;
   f32x4 acc[G::FM][G::FN];
-  gemm_loop<G>(g, m0, n0, s0, s1, steps, z, ldsA0, ldsB0, ldsA1, ldsB1, wm, wn, lane, acc);
+  Core<T, BM, BN, WM, WN, A_KO, B_KO, PAIR>::run(g, m0, n0, s0, s1, steps, z, wm, wn, lane, acc);
 #pragma unroll
   for (int i = 0; i < G::FM; i++) {
     const int64_t m = m0 + wm * (BM / WM) + 16 * i + (lane & 15);
@@ -290,7 +309,7 @@ template <typename T, int ACT, bool BWD>
 static int launch_gated(int64_t rows, int64_t D, int64_t F, const Operands<T> &op, const GatedOut &out, hipStream_t st) {
   constexpr int kK = kStepBytes / (int)sizeof(T);
   const int64_t cols = BWD ? out.ldo : F;
-  constexpr bool kWide = sizeof(T) == 2 || !BWD;  // (32 bits: forward 417 -> 369 us of 169343 x 128 x 512, backward 488 -> 523)
+  constexpr bool kWide = sizeof(T) == 2;  // (32 bits: three planes of 256 + 256 rows leave no room for a second workgroup)
   const TilePlan p = tile_plan(rows, cols, (D + kK - 1) / kK, 1, true, kWide, false);
   GemmArgs g = {{op.x, nullptr}, {op.wg, op.wu}, op.ldx * (int64_t)sizeof(T), op.ldw * (int64_t)sizeof(T), rows, F, D, p.tiles_m, p.tiles_n, 1};
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n));

@@ -8,10 +8,11 @@
 //     this step's matrix instructions run.  Rows and K values behind the matrix read as zeros (their lanes ask for an offset behind the
 //     descriptor's range).
 //   * LDS -> registers: 16 bytes a lane = 16 rows x 64 bytes of K ("slice") for one 16 x 16 x (64 bytes) matrix step.  K-inner tiles are
-//     read with ds_read_b128, K-outer tiles with the transposing ds_read_b64_tr_b16 (16-bit types) or dword reads (32-bit).
+//     read with ds_read_b128, K-outer tiles with the transposing ds_read_b64_tr_b16.
 //   * The 16-byte pieces of an LDS row are permuted (XOR with some bits of the row), so that the rows that are read together lie in
 //     different banks; the loads fetch the pieces in that order, the LDS side of a load being a straight line by construction.
 //   * The operands enter the matrix instruction as (B, A): a lane then holds four neighbouring n of one row m, which leave in one store.
+// 32-bit operands take another way to LDS (Gemm3 below): through registers, where each value becomes three of 16 bits.
 // Sums are held in 32 bits throughout; K is walked in order, so a result depends on the tile shape and the number of splits alone, and
 // these on the sizes alone.
 #pragma once
@@ -63,46 +64,10 @@ __device__ __forceinline__ void multiply(const Slice (&a)[FM], const Slice (&b)[
       }
 }
 
-// A 32-bit value as three of 16 bits (bf16: 8 bits of mantissa each, the range of 32 bits): x = hi + mid + lo but for 2^-27 x, each rounded to
-// nearest from what is left.  A product of two such values is six products of their parts, the ones below 2^-26 of it left out: as close
-// as a product rounded to 32 bits, on matrix instructions that take the six (96 cycles for 16 x 16 x 32) in less than half the time of the
-// 32-bit ones (256).  The parts' products are exact, their sums held in 32 bits.  What differs: an infinity becomes a NaN (inf - inf).
-//
-// What is left of a value is one instruction, the dot product of its pair's parts with (-1, 0) or (0, -1) added to it: exact, like the
-// subtraction it stands for, without the part widened to 32 bits first (7 instructions a pair for the three parts, not 11).  The constants
-// are kept in registers: as inline constants these instructions take them for both halves.
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-struct Three {
-  bf16x8 p[3];
-};
-struct Minus {  // (-1, 0) and (0, -1) in bf16
-  uint32_t lo = 0x0000bf80u, hi = 0xbf800000u;
-  __device__ __forceinline__ Minus() { asm volatile("" : "+s"(lo), "+s"(hi)); }
-};
-__device__ __forceinline__ void split3(const Slice &x0, const Slice &x1, const Minus &minus, Three &t) {
-  union { bf16x8 v; uint32_t u[4]; } p[3];
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const float *x = k < 2 ? x0.f + 2 * k : x1.f + 2 * k - 4;
-    f32x2 r = {x[0], x[1]};
-#pragma unroll
-    for (int q = 0; q < 3; q++) {
-      const bf16x2 h = __builtin_convertvector(r, bf16x2);
-      p[q].u[k] = __builtin_bit_cast(uint32_t, h);
-      if (q < 2) {
-        r[0] = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, minus.lo), r[0], false);
-        r[1] = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, minus.hi), r[1], false);
-      }
-    }
-  }
-#pragma unroll
-  for (int q = 0; q < 3; q++) t.p[q] = p[q].v;
-}
-
 // ---- one operand's tile in LDS: R rows (of M or N) x 128 bytes of K, R * 128 bytes -------------------------------------------------
 template <typename T, int R, bool KO>
 struct Tile {
+  static_assert(sizeof(T) == 2 || (sizeof(T) == 1 && !KO), "32-bit operands: Planes");
   static constexpr int kBytes = R * kStepBytes;
   static constexpr int kK = kStepBytes / (int)sizeof(T);       // K values a step
   static constexpr int kCpr = KO ? R * (int)sizeof(T) / 16 : 8;  // 16-byte pieces of an LDS row (K-outer: a row is one k)
@@ -110,8 +75,7 @@ struct Tile {
   // which piece of the row the LDS place `slot` holds (and the other way round): rows that are read together go to different banks
   static __device__ __forceinline__ int mix(int row, int slot) {
     if constexpr (!KO) return slot ^ ((row >> 1) & 7);
-    else if constexpr (sizeof(T) == 2) return slot ^ (2 * (((row & 3) + ((row >> 1) & 4)) & (kCpr / 2 - 1)));  // (4 rows and every second 8 rows are read together)
-    else return slot ^ (4 * ((row >> 2) & (kCpr / 4 - 1) & 3));
+    else return slot ^ (2 * (((row & 3) + ((row >> 1) & 4)) & (kCpr / 2 - 1)));  // (4 rows and every second 8 rows are read together)
   }
   // A thread loads pieces id, id + THREADS, ... (of R * 8, in LDS order): kRowsPerLoad rows apart, at the same place of the row where the
   // permutation does not change over that distance (kSame).
@@ -124,15 +88,14 @@ struct Tile {
   }
   template <int THREADS>
   static constexpr bool same() {
-    constexpr int rows = THREADS / kCpr;  // a load further
-    return !KO ? rows % 16 == 0 : sizeof(T) == 2 ? rows % 16 == 0 : rows % 16 == 0;
+    return THREADS / kCpr % 16 == 0;
   }
   // the slice of rows [16 i, 16 i + 16), 64 bytes kk of K
   static __device__ __forceinline__ void read(const char *lds, int row0, int kk, int lane, Slice &s) {
     if constexpr (!KO) {
       const int row = row0 + (lane & 15), slot = mix(row, (lane >> 4) + 4 * kk);
       s.u = *reinterpret_cast<const dgs_u4 *>(lds + row * kStepBytes + slot * 16);
-    } else if constexpr (sizeof(T) == 2) {
+    } else {
       // each 16 lanes read 4 k x 16 m (8 bytes a lane) and get them transposed: a lane has the 4 k of its m
       const int i = lane & 15;
 #pragma unroll
@@ -141,13 +104,6 @@ struct Tile {
         const int byte = row0 * 2 + (i & 3) * 8;
         const char *p = lds + k * (kCpr * 16) + mix(k, byte / 16) * 16 + byte % 16;
         s.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds_char *)p);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int k = 16 * kk + 4 * (lane >> 4) + j;
-        const int byte = (row0 + (lane & 15)) * 4;
-        s.f[j] = *reinterpret_cast<const float *>(lds + k * (kCpr * 16) + mix(k, byte / 16) * 16 + byte % 16);
       }
     }
   }
@@ -180,19 +136,24 @@ __device__ __forceinline__ Where where_of(int tiles_m, int tiles_n) {
   return {panel * kPanel + in % rows, in / rows, (int)blockIdx.y};
 }
 
-// The tile's sums: acc[i][j] = 16 x 16 at rows 16 i, columns col_of(j) of the wave's part; lane l register r holds m = l % 16, n = 4 (l / 16) + r.
-// STEP(i, j, part) is called for each 128 bytes of K where SCALED (8-bit types) instead of accumulating straight on.
-template <typename T, int BM, int BN, int WM, int WN, bool A_KO, bool B_KO, int PAIR>
-struct Gemm {
+// bytes from a tile's corner to the matrix's last row's end, as a descriptor's range
+__device__ __forceinline__ int tile_range(int64_t rows, int64_t ld) {
+  const int64_t b = rows * ld;
+  return b < kRange ? (int)b : kRange;
+}
+// The workgroup's waves meet: this wave's LDS accesses are done, loads to registers may be on their way.
+__device__ __forceinline__ void lds_meet() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// How a workgroup's waves share a tile
+template <int BM, int BN, int WM, int WN, int PAIR>
+struct Shares {
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
   static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  using TA = Tile<T, BM, A_KO>;
-  using TB = Tile<T, BN, B_KO>;
-  static constexpr int QA = BM * 8 / kThreads, QB = BN * 8 / kThreads;  // 16-byte loads of a thread a step
-  static constexpr int kCols = PAIR == kDual ? BN / 2 : BN;             // columns of C that a tile covers
-  static_assert(QA * kThreads == BM * 8 && QB * kThreads == BN * 8, "whole loads");
-  static_assert(PAIR != kDual || (!B_KO && QB % 2 == 0), "halves of the loads");
-
+  static constexpr int kCols = PAIR == kDual ? BN / 2 : BN;  // columns of C that a tile covers
   // column of the tile's B rows where the wave's j-th 16 columns begin, and the column of C
   static __device__ __forceinline__ int b_row(int wn, int j) {
     if constexpr (PAIR == kDual) return (j < FN / 2 ? 0 : BN / 2) + wn * (BN / 2 / WN) + 16 * (j % (FN / 2));
@@ -202,6 +163,19 @@ struct Gemm {
     if constexpr (PAIR == kDual) return wn * (BN / 2 / WN) + 16 * (j % (FN / 2));
     return wn * (BN / WN) + 16 * j;
   }
+};
+
+// The tile's sums: acc[i][j] = 16 x 16 at rows 16 i, columns col_of(j) of the wave's part; lane l register r holds m = l % 16, n = 4 (l / 16) + r.
+// STEP(i, j, part) is called for each 128 bytes of K where SCALED (8-bit types) instead of accumulating straight on.
+template <typename T, int BM, int BN, int WM, int WN, bool A_KO, bool B_KO, int PAIR>
+struct Gemm : Shares<BM, BN, WM, WN, PAIR> {
+  using S = Shares<BM, BN, WM, WN, PAIR>;
+  using S::FM, S::FN, S::b_row, S::kThreads, S::kWaves;
+  using TA = Tile<T, BM, A_KO>;
+  using TB = Tile<T, BN, B_KO>;
+  static constexpr int QA = BM * 8 / kThreads, QB = BN * 8 / kThreads;  // 16-byte loads of a thread a step
+  static_assert(QA * kThreads == BM * 8 && QB * kThreads == BN * 8, "whole loads");
+  static_assert(PAIR != kDual || (!B_KO && QB % 2 == 0), "halves of the loads");
 
   // One thread's share of a step's loads: the offset of the first, and of the others where they do not follow from it by the rows' distance.
   static constexpr bool kSameA = TA::template same<kThreads>(), kSameB = TB::template same<kThreads>();
@@ -227,11 +201,6 @@ struct Gemm {
     l.da = kThreads / TA::kCpr * (int)g.lda;
     l.db = kThreads / TB::kCpr * (int)g.ldb;
   }
-  // bytes from a tile's corner to the matrix's last row's end, as a descriptor's range
-  static __device__ __forceinline__ int range(int64_t rows, int64_t ld) {
-    const int64_t b = rows * ld;
-    return b < kRange ? (int)b : kRange;
-  }
   // The loads of step s (of `steps` a walk over K; kSum: 2 * steps in all) into one LDS buffer
   static __device__ __forceinline__ void load(const Load &l, const GemmArgs &g, int m0, int n0, int s, int steps, int z, char *la, char *lb) {
     const int seg = PAIR == kSum ? (s >= steps ? 1 : 0) : 0;
@@ -241,7 +210,7 @@ struct Gemm {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     {
       const char *p = g.A[PAIR == kTwo ? z : seg] + (A_KO ? k0 * g.lda + m0 * (int64_t)sizeof(T) : m0 * g.lda + k0 * (int64_t)sizeof(T));
-      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, range(A_KO ? kleft : g.M - m0, g.lda), 0x00027000);
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, tile_range(A_KO ? kleft : g.M - m0, g.lda), 0x00027000);
       const bool on = A_KO || l.ka < left;
 #pragma unroll
       for (int q = 0; q < QA; q++) {
@@ -252,7 +221,7 @@ struct Gemm {
 #pragma unroll
     for (int half = 0; half < (PAIR == kDual ? 2 : 1); half++) {
       const char *p = g.B[PAIR == kDual ? half : seg] + (B_KO ? k0 * g.ldb + n0 * (int64_t)sizeof(T) : n0 * g.ldb + k0 * (int64_t)sizeof(T));
-      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, range(B_KO ? kleft : g.N - n0, g.ldb), 0x00027000);
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, tile_range(B_KO ? kleft : g.N - n0, g.ldb), 0x00027000);
       const bool on = B_KO || l.kb < left;
 #pragma unroll
       for (int q = 0; q < PB; q++) {
@@ -262,32 +231,6 @@ struct Gemm {
     }
   }
   static __device__ __forceinline__ void compute(const char *la, const char *lb, int wm, int wn, int lane, f32x4 (&acc)[FM][FN]) {
-    if constexpr (sizeof(T) == 4) {
-      // (a lane's 8 values of K: 4 of each half of the step, the same in both operands)
-      const Minus minus;
-      Three b[FN];
-#pragma unroll
-      for (int j = 0; j < FN; j++) {
-        Slice x0, x1;
-        TB::read(lb, b_row(wn, j), 0, lane, x0);
-        TB::read(lb, b_row(wn, j), 1, lane, x1);
-        split3(x0, x1, minus, b[j]);
-      }
-#pragma unroll
-      for (int i = 0; i < FM; i++) {
-        Slice x0, x1;
-        Three a;
-        TA::read(la, wm * (BM / WM) + 16 * i, 0, lane, x0);
-        TA::read(la, wm * (BM / WM) + 16 * i, 1, lane, x1);
-        split3(x0, x1, minus, a);
-        constexpr int pa[6] = {0, 2, 1, 0, 1, 0}, pb[6] = {2, 0, 1, 1, 0, 0};  // the small ones first
-#pragma unroll
-        for (int q = 0; q < 6; q++)
-#pragma unroll
-          for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j].p[pb[q]], a.p[pa[q]], acc[i][j], 0, 0, 0);
-      }
-      return;
-    }
 #pragma unroll
     for (int kk = 0; kk < 2; kk++) {
       __builtin_amdgcn_sched_barrier(0);  // (one half's operands in registers at a time)
@@ -308,7 +251,7 @@ __device__ __forceinline__ void loads_done() {
   __syncthreads();
 }
 
-// The main loop, 16- and 32-bit types: steps [s0, s1) into acc.  The four LDS buffers are separate arrays, so that the compiler sees that
+// The main loop, 16-bit types: steps [s0, s1) into acc.  The four LDS buffers are separate arrays, so that the compiler sees that
 // a step's reads and the next step's loads do not meet and does not wait for the loads in between.
 #define DGS_GEMM_LDS(G)                                              \
   __shared__ __align__(16) char ldsA0[G::TA::kBytes], ldsB0[G::TB::kBytes]; \
@@ -337,6 +280,166 @@ __device__ __forceinline__ void gemm_loop(const GemmArgs &g, int m0, int n0, int
   }
   if (s < s1) G::compute(ldsA0, ldsB0, wm, wn, lane, acc);
 }
+
+// ---- 32-bit operands ----------------------------------------------------------------------------------------------------------
+// A 32-bit value as three of 16 bits (bf16: 8 bits of mantissa each, the range of 32 bits): x = hi + mid + lo but for 2^-27 x, each rounded to
+// nearest from what is left.  A product of two such values is six products of their parts, the ones below 2^-26 of it left out: as close
+// as a product rounded to 32 bits, on matrix instructions that take the six (96 cycles for 16 x 16 x 32) in less than half the time of the
+// 32-bit ones (256).  The parts' products are exact, their sums held in 32 bits.  What differs: an infinity becomes a NaN (inf - inf).
+//
+// What is left of a value is one instruction, the dot product of its pair's parts with (-1, 0) or (0, -1) added to it: exact, like the
+// subtraction it stands for, without the part widened to 32 bits first (7 instructions a pair for the three parts, not 11).  The constants
+// are kept in registers: as inline constants these instructions take them for both halves.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+struct Minus {  // (-1, 0) and (0, -1) in bf16
+  uint32_t lo = 0x0000bf80u, hi = 0xbf800000u;
+  __device__ __forceinline__ Minus() { asm volatile("" : "+s"(lo), "+s"(hi)); }
+};
+__device__ __forceinline__ void split3(f32x2 r, const Minus &minus, uint32_t (&part)[3]) {
+#pragma unroll
+  for (int q = 0; q < 3; q++) {
+    const bf16x2 h = __builtin_convertvector(r, bf16x2);
+    part[q] = __builtin_bit_cast(uint32_t, h);
+    if (q < 2) {
+      r[0] = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, minus.lo), r[0], false);
+      r[1] = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, minus.hi), r[1], false);
+    }
+  }
+}
+
+// One operand's step of 32 K values in LDS: three planes of R rows x 64 bytes (K-inner) or 32 rows x 2 R bytes (K-outer).
+template <int R, bool KO>
+struct Planes {
+  static constexpr int kPlane = R * 64, kBytes = 3 * kPlane;
+  static constexpr int kPieces = KO ? R / 4 : 8;  // 16-byte pieces (4 values) of a row in memory
+  using Outer = Tile<bf16, R, true>;
+  static __device__ __forceinline__ uint32_t offset(int id, int64_t ld, int64_t left, int &k) {
+    const int row = id / kPieces, piece = id % kPieces;
+    k = KO ? 0 : 4 * piece;
+    return !KO || piece * 16 < left ? (uint32_t)(row * (int)ld + piece * 16) : kNowhere;
+  }
+  static __device__ __forceinline__ int mix(int row, int slot) {
+    if constexpr (KO) return Outer::mix(row, slot);
+    else return slot ^ (-(row >> 2) & 3);  // (the 16 lanes that read together take rows 0-3, 12-15 of one piece and 4-7, 8-11 of the next)
+  }
+  // piece `id` of the step (4 neighbouring values), split, into the planes
+  static __device__ __forceinline__ void write(char *lds, int id, const f32x4 &x, const Minus &minus) {
+    const int row = id / kPieces, piece = id % kPieces;
+    uint32_t p[2][3];
+#pragma unroll
+    for (int h = 0; h < 2; h++) split3(f32x2{x[2 * h], x[2 * h + 1]}, minus, p[h]);
+    char *at = lds + row * (KO ? 2 * R : 64) + mix(row, piece / 2) * 16 + piece % 2 * 8;
+#pragma unroll
+    for (int q = 0; q < 3; q++) *reinterpret_cast<dgs_u2 *>(at + q * kPlane) = dgs_u2{p[0][q], p[1][q]};
+  }
+  // The 16 rows at row0, a multiple of 16: lane group g has K values 8 g .. 8 g + 7.  `Place`: where the lane reads of a plane at row 0; row0 is added
+  // (K-outer: a bit of the place within the LDS row, which the permutation leaves as it is, or turns: an exclusive or).
+  struct Place { uint32_t at[KO ? 2 : 1]; };
+  static __device__ __forceinline__ Place place(int lane) {
+    Place p;
+    if constexpr (!KO) {
+      p.at[0] = (lane & 15) * 64 + mix(lane & 15, lane >> 4) * 16;
+    } else {
+      const int i = lane & 15;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int k = 8 * (lane >> 4) + 4 * h + (i >> 2);
+        p.at[h] = k * 2 * R + mix(k, (i & 3) / 2) * 16 + (i & 1) * 8;
+      }
+    }
+    return p;
+  }
+  static __device__ __forceinline__ void read(const char *plane, const Place &p, int row0, Slice &s) {
+    if constexpr (!KO) {
+      s.u = *reinterpret_cast<const dgs_u4 *>(plane + p.at[0] + row0 * 64);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        s.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds_char *)(plane + (p.at[h] ^ (row0 * 2))));
+    }
+  }
+};
+
+template <int BM, int BN, int WM, int WN, bool A_KO, bool B_KO, int PAIR>
+struct Gemm3 : Shares<BM, BN, WM, WN, PAIR> {
+  using S = Shares<BM, BN, WM, WN, PAIR>;
+  using S::FM, S::FN, S::b_row, S::kThreads;
+  static constexpr int kK = 32;
+  using PA = Planes<BM, A_KO>;
+  using PB = Planes<BN, B_KO>;
+  static constexpr int QA = BM * 8 / kThreads, QB = BN * 8 / kThreads, PBQ = PAIR == kDual ? QB / 2 : QB;  // (as in Gemm)
+  static_assert(kThreads % PA::kPieces == 0 && kThreads % PB::kPieces == 0, "a thread's pieces lie below each other");
+  struct Raw { f32x4 a[QA], b[QB]; };
+  struct Load { uint32_t a, b; int ka, kb; };
+  static __device__ __forceinline__ void load(const Load &l, const GemmArgs &g, int m0, int n0, int s, int steps, int z, Raw &raw) {
+    const int seg = PAIR == kSum ? (s >= steps ? 1 : 0) : 0;
+    const int64_t k0 = (int64_t)(s - seg * steps) * kK, kleft = g.K - k0;
+    const int left = (int)(kleft < kK ? kleft : kK);
+    {
+      const char *p = g.A[PAIR == kTwo ? z : seg] + (A_KO ? k0 * g.lda + m0 * (int64_t)4 : m0 * g.lda + k0 * (int64_t)4);
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, tile_range(A_KO ? kleft : g.M - m0, g.lda), 0x00027000);
+      const bool on = A_KO || l.ka < left;
+#pragma unroll
+      for (int q = 0; q < QA; q++)
+        raw.a[q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, on ? (int)(l.a + (uint32_t)(q * (kThreads / PA::kPieces) * (int)g.lda)) : (int)kNowhere, 0, 0));
+    }
+#pragma unroll
+    for (int half = 0; half < (PAIR == kDual ? 2 : 1); half++) {
+      const char *p = g.B[PAIR == kDual ? half : seg] + (B_KO ? k0 * g.ldb + n0 * (int64_t)4 : n0 * g.ldb + k0 * (int64_t)4);
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, tile_range(B_KO ? kleft : g.N - n0, g.ldb), 0x00027000);
+      const bool on = B_KO || l.kb < left;
+#pragma unroll
+      for (int q = 0; q < PBQ; q++)
+        raw.b[half * PBQ + q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, on ? (int)(l.b + (uint32_t)(q * (kThreads / PB::kPieces) * (int)g.ldb)) : (int)kNowhere, 0, 0));
+    }
+  }
+  // Steps [s0, s1) into acc.  The next step's operands are on their way to registers while this one's, split, are multiplied out of LDS: each
+  // value is split once for the workgroup, not by each of the two waves that read it (169343 x 128 x 512, forward and backward: 1316 -> 1182 us),
+  // and one buffer of 48 KB leaves room for three workgroups on a CU, which fill each other's waits at the two barriers of a step.
+  static __device__ __forceinline__ void run(const GemmArgs &g, int m0, int n0, int s0, int s1, int steps, int z, char *lds, int wm, int wn, int lane, f32x4 (&acc)[FM][FN]) {
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+      for (int j = 0; j < FN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (s0 >= s1) return;
+    const Minus minus;
+    const typename PA::Place placeA = PA::place(lane);
+    const typename PB::Place placeB = PB::place(lane);
+    const int t = (int)threadIdx.x;
+    Load l;
+    l.a = PA::offset(t, g.lda, ((g.M - m0) * 4 + 15) / 16 * 16, l.ka);
+    l.b = PB::offset(t, g.ldb, ((g.N - n0) * 4 + 15) / 16 * 16, l.kb);
+    Raw raw;
+    load(l, g, m0, n0, s0, steps, z, raw);
+    char *la = lds, *lb = lds + PA::kBytes;
+    for (int s = s0; s < s1; s++) {
+      lds_meet();  // (the step before has been read)
+#pragma unroll
+      for (int q = 0; q < QA; q++) PA::write(la, q * kThreads + t, raw.a[q], minus);
+#pragma unroll
+      for (int q = 0; q < QB; q++) PB::write(lb, q * kThreads + t, raw.b[q], minus);
+      load(l, g, m0, n0, s + 1 < s1 ? s + 1 : s, steps, z, raw);  // (the last step's again, unused: a branch round the loads is slower, 1205 us for 1185)
+      lds_meet();
+      Slice b[FN][3];
+#pragma unroll
+      for (int j = 0; j < FN; j++)
+#pragma unroll
+        for (int q = 0; q < 3; q++) PB::read(lb + q * PB::kPlane, placeB, b_row(wn, j), b[j][q]);
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+        Slice a[3];
+#pragma unroll
+        for (int q = 0; q < 3; q++) PA::read(la + q * PA::kPlane, placeA, wm * (BM / WM) + 16 * i, a[q]);
+        constexpr int pa[6] = {0, 2, 1, 0, 1, 0}, pb[6] = {2, 0, 1, 1, 0, 0};  // the small ones first
+#pragma unroll
+        for (int q = 0; q < 6; q++)
+#pragma unroll
+          for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j][pb[q]].b, a[pa[q]].b, acc[i][j], 0, 0, 0);
+      }
+    }
+  }
+};
 
 // four neighbouring columns of a row; `vec`: the row's stride and base allow one store
 template <typename T>
