@@ -2,10 +2,12 @@
 //
 //   out[m, n] = sum over blocks b of 128 k:  sa[m, b] sb[n / 128, b]  sum over k in b of a[m, k] b[n, k]
 //
-// A step of 128 bytes of K is one block: one 16 x 16 x 128 matrix instruction from a zero start gives the inner sum, one multiply-add with the two scales' product adds it to the running sum in 32 bits.  The operands'
-// order in the instruction puts m on the lanes, so a lane needs one scale of a for each 16 rows; a wave's columns lie within one block of
-// 128, so the scale of b is the wave's.
+// A step of 128 bytes of K is one block: one 16 x 16 x 128 matrix instruction from a zero start gives the inner sum, one multiply-add with
+// the two scales' product adds it to the running sum in 32 bits.  The operands' order in the instruction puts m on the lanes, so a lane
+// needs one scale of a for each 16 rows; a wave's columns lie within one block of 128, so the scale of b is the wave's.
 // Bound: many rows: the matrix cores, with four multiply-adds a lane beside each instruction; few rows: the bytes of b (fp8_few_kernel).
+// Measured: 4095 x 11000 x 4096, bf16 out: 196 - 215 us (1.7 - 1.9 PFLOP/s; a large product without block scales, the library's: 2.7);
+// 5 x 4096 x 11008: 13.3 us a call (45 MB: 3.4 TB/s).
 #include "gemm_core.h"
 
 namespace dgs {

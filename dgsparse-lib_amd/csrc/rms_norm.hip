@@ -8,6 +8,8 @@
 //
 // Bound: HBM.  Forward reads 2 rows and writes 2, backward reads 3 and writes 1; a row is read once and stays in registers between its
 // reduction and its use (NV 16-byte vectors per lane).  Row statistics and dw are sums in 32 bits.
+// Measured (kernel time; a large copy runs at 5.1 TB/s):  8192 x 4096 bf16 forward 50 us (5.3 TB/s), backward 55 (4.9) and 10 for dw's join;
+// 169343 x 128 fp32 57 (6.1, part of it out of the last cache), 73 (4.7) and 11;  8-bit output, 8191 x 5120 fp16, 59 us (5.0 TB/s).
 #include "dense_common.h"
 
 namespace dgs {
