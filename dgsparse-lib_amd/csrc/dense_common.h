@@ -87,6 +87,8 @@ __device__ __forceinline__ float group_sum(float x, float *red) {
   return x;
 }
 
+// a launch's threads in one dimension are counted in 32 bits
+inline bool grid_ok(int64_t blocks, int64_t threads = kBlock) { return blocks * threads <= 0xffffffffll; }
 inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 inline size_t dtype_bytes(int dtype) { return dtype == DGS_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == DGS_F32 || dtype == DGS_F16 || dtype == DGS_BF16; }

@@ -396,6 +396,7 @@ static int fwd(int64_t n, int64_t V, int64_t D, const void *ids, const void *tab
   const bool vec = D % kVec<T> == 0 && ld % kVec<T> == 0 && aligned_to(table, 16) && aligned_to(out, 16);
   const int G = lanes_for((D + kVec<T> - 1) / kVec<T>);
   const int64_t blocks = (n + kBlock / G - 1) / (kBlock / G);
+  if (!grid_ok(blocks)) return DGS_ERANGE;
   if (vec)
     hipLaunchKernelGGL((embedding_fwd_kernel<T, I, true>), dim3((unsigned)blocks), dim3(kBlock), 0, st, n, V, (int)D, G, (const I *)ids, (const T *)table, ld, scale, (T *)out);
   else
@@ -441,7 +442,7 @@ static int bwd(int64_t n, int64_t V, int64_t D, const uint32_t *key, const int *
   const int64_t rowb = D * (int64_t)sizeof(T);
   const int fill_rows = (int)(65536 / rowb < 1 ? 1 : 65536 / rowb > 256 ? 256 : 65536 / rowb);
   const int64_t fill = (V + fill_rows - 1) / fill_rows, work = (n_chunks + per - 1) / per * tiles;
-  if (fill + work > INT32_MAX) return DGS_ERANGE;
+  if (!grid_ok(fill + work)) return DGS_ERANGE;
   // zeros past the caches up to the last level's 256 MB (an 87 MB table: 46 us, through them 52), through them beyond (1 GB: 219 us, past 249)
   const int keep = V * rowb > ((int64_t)256 << 20);
   const dim3 grid((unsigned)(work + fill));
@@ -477,7 +478,7 @@ extern "C" int dgs_embedding(int dtype, int id_bytes, int64_t n, int64_t V, int6
   const int rc = embedding_sizes(dtype, id_bytes, n, V, D);
   if (rc != DGS_OK) return rc;
   if (n == 0) return DGS_OK;
-  if (!ids || !out || (V > 0 && !table)) return DGS_EINVAL;
+  if (!ids || !out || (V > 0 && !table) || ld_table < 0) return DGS_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define DGS_GO(T) return id_bytes == 8 ? fwd<T, int64_t>(n, V, D, ids, table, ld_table, scale, out, st) : fwd<T, int32_t>(n, V, D, ids, table, ld_table, scale, out, st)
   if (dtype == DGS_F32) DGS_GO(float);
@@ -496,7 +497,7 @@ extern "C" int dgs_embedding_bwd(int dtype, int id_bytes, int64_t n, int64_t V, 
   const int rc = embedding_sizes(dtype, id_bytes, n, V, D);
   if (rc != DGS_OK) return rc;
   if (V == 0) return DGS_OK;
-  if (!dtable || (n > 0 && (!ids || !dout))) return DGS_EINVAL;
+  if (!dtable || (n > 0 && (!ids || !dout || ld_dout < 0))) return DGS_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
   uint32_t *key = nullptr;
   int *pos = nullptr;

@@ -306,7 +306,7 @@ template <typename T>
 static int quantize(int64_t rows, int64_t cols, const void *x, int64_t ld, int block_rows, uint8_t *q, float *scales, hipStream_t st) {
   const bool vec = ld % 4 == 0 && aligned_to(x, 4 * sizeof(T));
   const int64_t blocks = (cols + 127) / 128, grid = block_rows == 1 ? (rows * blocks + 7) / 8 : (rows + 127) / 128 * blocks;
-  if (grid > INT32_MAX) return DGS_ERANGE;
+  if (!grid_ok(grid)) return DGS_ERANGE;
   if (block_rows == 1)
     hipLaunchKernelGGL((quantize_kernel<T, 1>), dim3((unsigned)grid), dim3(kBlock), 0, st, rows, cols, (const T *)x, ld, vec, q, scales);
   else
@@ -350,6 +350,7 @@ static int matmul8(int64_t M, int64_t N, int64_t K, const void *a, int64_t lda, 
   }
   const Scales sc = {sa, sb, (K + 127) / 128};
   if (M <= kFewRows8) {
+    if (!grid_ok((N + 15) / 16, 512)) return DGS_ERANGE;
     const dim3 grid((unsigned)((N + 15) / 16));
     if (M <= 16) hipLaunchKernelGGL((fp8_few_kernel<T, 1>), grid, dim3(512), 0, st, ap, lda, bp, ldb, (int)M, N, L.ldk, sc, out);
     else if (M <= 32) hipLaunchKernelGGL((fp8_few_kernel<T, 2>), grid, dim3(512), 0, st, ap, lda, bp, ldb, (int)M, N, L.ldk, sc, out);
@@ -359,6 +360,7 @@ static int matmul8(int64_t M, int64_t N, int64_t K, const void *a, int64_t lda, 
   const TilePlan &p = L.plan;
   float *partial = p.splits > 1 ? (float *)(ws + L.partial) : nullptr;
   const GemmArgs g = {{ap, nullptr}, {bp, nullptr}, lda, ldb, M, N, L.ldk, p.tiles_m, p.tiles_n, p.splits};
+  if (!grid_ok((int64_t)p.tiles_m * p.tiles_n, p.shape == kBig ? 512 : 256)) return DGS_ERANGE;
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits);
   bool done = false;
   if constexpr (sizeof(T) == 2) {
@@ -409,7 +411,7 @@ extern "C" int dgs_matmul_fp8(int out_dtype, int64_t M, int64_t N, int64_t K, co
   if (M == 0 || N == 0) return DGS_OK;
   if (!a || !a_scale || !b || !b_scale || !out || !aligned_to(out, 16)) return DGS_EINVAL;
   // (K a multiple of 16: the operands are read in place, 16 bytes at a time)
-  if (K % 16 == 0 && (!aligned_to(a, 16) || !aligned_to(b, 16) || lda % 16 || ldb % 16)) return DGS_EINVAL;
+  if (K % 16 == 0 && (!aligned_to(a, 16) || !aligned_to(b, 16) || lda % 16 || ldb % 16 || lda < K || ldb < K)) return DGS_EINVAL;
   const size_t need = dgs_matmul_fp8_workspace_bytes(M, N, K);
   if (need && (!workspace || workspace_bytes < need)) return DGS_EWORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);

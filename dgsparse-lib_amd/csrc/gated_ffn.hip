@@ -315,6 +315,7 @@ static int launch_gated(int64_t rows, int64_t D, int64_t F, const Operands<T> &o
   constexpr bool kWide = sizeof(T) == 2;  // (32 bits: three planes of 256 + 256 rows leave no room for a second workgroup)
   const TilePlan p = tile_plan(rows, cols, (D + kK - 1) / kK, 1, true, kWide, false);
   GemmArgs g = {{op.x, nullptr}, {op.wg, op.wu}, op.ldx * (int64_t)sizeof(T), op.ldw * (int64_t)sizeof(T), rows, F, D, p.tiles_m, p.tiles_n, 1};
+  if (!grid_ok((int64_t)p.tiles_m * p.tiles_n, p.shape == kBig ? 512 : 256)) return DGS_ERANGE;
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n));
   if constexpr (kWide) {
     if (p.shape == kBig) {
@@ -335,6 +336,7 @@ static int launch_product(GemmArgs g, PlainOut o, const TilePlan &p, float *part
   g.tiles_n = p.tiles_n;
   g.splits = p.splits;
   o.partial = p.splits > 1 ? partial : nullptr;
+  if (!grid_ok((int64_t)p.tiles_m * p.tiles_n, p.shape == kBig ? 512 : 256)) return DGS_ERANGE;
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)(p.splits * mats));
   bool done = false;
   if constexpr (sizeof(T) == 2) {
@@ -365,6 +367,7 @@ static int ffn_fwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ld
   const int rc = operands<T>(rows, D, F, x, ldx, wg, wu, ldw, ws, L, st, op);
   if (rc != DGS_OK) return rc;
   if (rows <= kFewRows) {
+    if (!grid_ok((F + 15) / 16, 512)) return DGS_ERANGE;
     const dim3 grid((unsigned)((F + 15) / 16));
     const int64_t kb = (int64_t)(L.pad ? L.ldx : D) * (int64_t)sizeof(T), lx = op.ldx * (int64_t)sizeof(T), lw = op.ldw * (int64_t)sizeof(T);
 #define DGS_FEW(FM_) hipLaunchKernelGGL((gated_few_kernel<T, FM_, ACT>), grid, dim3(512), 0, st, op.x, lx, op.wg, op.wu, lw, (int)rows, F, kb, (T *)h, pre)
@@ -392,7 +395,9 @@ static int ffn_bwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ld
   if (pre) {
     int G = 1;
     while (G < kBlock && G * kVec<T> < F) G <<= 1;
-    const dim3 grid((unsigned)((rows + kBlock / G - 1) / (kBlock / G)));
+    const int64_t blocks = (rows + kBlock / G - 1) / (kBlock / G);
+    if (!grid_ok(blocks)) return DGS_ERANGE;
+    const dim3 grid((unsigned)blocks);
     if (F % kVec<T> == 0)
       hipLaunchKernelGGL((gated_split_kernel<T, ACT, true>), grid, dim3(kBlock), 0, st, rows, G, out);
     else

@@ -494,7 +494,7 @@ __global__ __launch_bounds__(kBlock) void pad_rows_kernel(int64_t rows, int64_t 
 template <typename T>
 static int pad_rows(int64_t rows, int64_t cols, const void *src, int64_t ld, int64_t ldo, void *dst, hipStream_t st) {
   const int64_t n = rows * (ldo * (int64_t)sizeof(T) / 16), blocks = (n + kBlock - 1) / kBlock;
-  if (blocks > INT32_MAX) return DGS_ERANGE;
+  if (!grid_ok(blocks)) return DGS_ERANGE;
   hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)blocks), dim3(kBlock), 0, st, rows, cols, (const T *)src, ld, ldo, (T *)dst);
   return check_launch();
 }

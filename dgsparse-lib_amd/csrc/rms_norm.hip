@@ -303,6 +303,7 @@ static int launch_norm(int64_t rows, int D, const T *x, int64_t ldx, const T *re
                        float *scales, hipStream_t st) {
   const NormShape sh = norm_shape((D + kVec<T> - 1) / kVec<T>, FP8 ? 128 / kVec<T> : 8);
   const int64_t blocks = (rows + kBlock / sh.G - 1) / (kBlock / sh.G);
+  if (!grid_ok(blocks)) return DGS_ERANGE;
 #define DGS_NORM(G_, NV_)                                                                                                              \
   if (sh.G == G_ && sh.NV == NV_) {                                                                                                    \
     hipLaunchKernelGGL((rms_norm_kernel<T, VECTOR, G_, NV_, RES, FP8>), dim3((unsigned)blocks), dim3(kBlock), 0, st, rows, D, x, ldx, res, ldr, w, \
@@ -381,6 +382,7 @@ static int norm_bwd(int64_t rows, int64_t D, const void *s, const void *w, float
   float *partial = (float *)ws;
   int64_t parts = 0;
   if (sh.NV == 0) {
+    if (!grid_ok(rows)) return DGS_ERANGE;
     float *rstd = (float *)ws;
     partial = (float *)(ws + round_up((size_t)rows * 4, 256));
     if (ds)
@@ -423,7 +425,7 @@ static bool norm_sizes_ok(int64_t rows, int64_t D) { return rows <= INT32_MAX &&
 
 extern "C" int dgs_rms_norm(int dtype, int64_t rows, int64_t D, const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *weight,
                             float eps, void *y, void *s, uint8_t *q, float *scales, dgsStream_t stream) {
-  if (!dtype_ok(dtype) || rows < 0 || D <= 0 || !(eps >= 0.0f)) return DGS_EINVAL;
+  if (!dtype_ok(dtype) || rows < 0 || D <= 0 || ldx < 0 || (residual && ldr < 0) || !(eps >= 0.0f)) return DGS_EINVAL;
   if (!norm_sizes_ok(rows, D)) return DGS_ERANGE;
   if (rows == 0) return DGS_OK;
   if (!x || !weight || (residual && !s) || (!residual && s) || (!y == !q) || (!q != !scales)) return DGS_EINVAL;

@@ -69,7 +69,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activat
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
     r"""``x`` [..., features] in 8 bits -> ``(q, scale)``: ``q`` in ``float8_e4m3fn`` and a float32 ``scale = max |x| / 448`` for each
-    ``block_rows`` x 128 values; ``x`` is ``q * scale``.  ``block_rows=1`` (a scale for each row: activations) or ``128`` (weights; 2-D)."""
+    ``block_rows`` x 128 values; ``x`` is ``q * scale``.  ``block_rows=1`` (a scale for each row: activations) or ``128`` (weights; 2-D).
+    It records no gradient."""
     if block_rows not in (1, 128):
         raise ValueError(f'dgsparse: block_rows must be 1 or 128, not {block_rows}')
     return _quantize_fp8(x, block_rows)

@@ -74,7 +74,8 @@ class LinearFP8(torch.nn.Module):
 class ResidualGCN(torch.nn.Module):
     """A residual graph layer with its norms in front: ``m = relu(A_hat (norm(x + r) W))``, ``out = ffn(norm(m + s))`` -> ``(out, s')`` where ``s``, ``s'``
     are the running residuals.  ``quantize()`` puts the graph projection into 8 bits for serving: the norm then writes 8-bit rows, which the
-    projection reads as they are."""
+    projection reads as they are.  The 8-bit weight is made once from the weight of that moment: training drops it, and after
+    ``load_state_dict`` it is to be made again."""
 
     def __init__(self, size: int, hidden_size: int, activation: str = 'silu', eps: float = 1e-6):
         super().__init__()
@@ -87,8 +88,13 @@ class ResidualGCN(torch.nn.Module):
         self.conv8 = LinearFP8(self.conv.W.weight)
         return self.eval()
 
+    def train(self, mode: bool = True) -> 'ResidualGCN':
+        if mode:
+            self.conv8 = None
+        return super().train(mode)
+
     def forward(self, dcsr, x: torch.Tensor, residual: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-        if self.conv8 is not None and not self.training:
+        if self.conv8 is not None:
             with torch.no_grad():
                 q, scale, s = dense.add_rms_norm_fp8(x, residual, self.norm1.weight, self.norm1.eps)
                 m = spmm_sum_fused(dcsr, self.conv8((q, scale)), relu=True)

@@ -95,6 +95,40 @@ def test_fp8_entries_refuse(lib):
     assert call(K=33, wsb=lib.dgs_matmul_fp8_workspace_bytes(4, 8, 33) - 1) == EWORKSPACE
 
 
+def test_rows_that_overlap_or_run_backwards_and_grids_beyond_32_bits_are_refused(lib):
+    # (an 8-bit operand that is read in place: a row distance below the row's length would end the last row early)
+    good = dict(dtype=BF16, M=4, N=8, K=32, a=P, lda=32, sa=P, b=P, ldb=32, sb=P, out=P, ws=P, wsb=1 << 30, stream=None)
+    for bad in (dict(lda=16), dict(ldb=16), dict(lda=0), dict(ldb=0)):
+        assert lib.dgs_matmul_fp8(*{**good, **bad}.values()) == EINVAL, bad
+    assert lib.dgs_matmul_fp8(*{**good, **dict(N=2 ** 27 + 64, wsb=1 << 62)}.values()) == ERANGE
+    good = dict(dtype=F16, rows=4, D=8, x=P, ldx=8, res=P, ldr=8, w=P, eps=1e-6, y=P, s=P, q=None, sc=None, stream=None)
+    for bad in (dict(ldx=-8), dict(ldr=-8)):
+        assert lib.dgs_rms_norm(*{**good, **bad}.values()) == EINVAL, bad
+    assert lib.dgs_rms_norm(*{**good, **dict(rows=2 ** 25, D=4096, ldx=4096, ldr=4096)}.values()) == ERANGE
+    good = dict(dtype=F32, idb=8, n=4, V=10, D=8, ids=P, table=P, ld=-8, scale=1.0, out=P, stream=None)
+    assert lib.dgs_embedding(*good.values()) == EINVAL
+    assert lib.dgs_embedding(*{**good, **dict(ld=4096, D=4096, n=2 ** 25)}.values()) == ERANGE
+    good = dict(dtype=BF16, idb=4, n=4, V=10, D=8, ids=P, pad=-1, dout=P, ld=-8, scale=1.0, dtable=P, ws=P, wsb=1 << 30, stream=None)
+    assert lib.dgs_embedding_bwd(*good.values()) == EINVAL
+    assert lib.dgs_quantize_fp8(F16, 2 ** 30, 128, P, 128, 1, P, P, None) == ERANGE
+    good = dict(dtype=BF16, act=0, rows=4, D=8, F=2 ** 23 - 2 ** 10, x=P, ldx=8, wg=P, wu=P, ldw=8, h=P, pre=None, ws=P, wsb=1 << 30, stream=None)
+    assert lib.dgs_gated_ffn(*{**good, **dict(F=2 ** 23)}.values()) == ERANGE
+
+
+def test_an_8_bit_projection_ends_with_the_weight_it_was_made_of(monkeypatch):
+    """Training drops it: the layer would go on with the projection of the old weight after the next eval()."""
+    import dgsparse.nn as nn
+    from dgsparse.nn import dense as layers
+    monkeypatch.setattr(layers.dense, 'quantize_fp8', lambda x, rows=1: (x.clone(), torch.ones(1, 1)))
+    layer = nn.ResidualGCN(8, 16).quantize()
+    assert layer.conv8 is not None and not layer.training
+    layer.eval()
+    assert layer.conv8 is not None
+    layer.train()
+    assert layer.conv8 is None
+    assert layer.eval().conv8 is None
+
+
 def test_python_functions_refuse():
     import dgsparse
     x, w, ids = torch.rand(4, 8), torch.rand(8), torch.zeros(3, dtype=torch.long)
