@@ -59,6 +59,7 @@ def _dgs_tuning_follows_env(monkeypatch):
     except Exception:  # CPU-only collection of tests that never import the package
         yield
         return
+    before = {k: v for k, v in os.environ.items() if k.startswith('DGS_')}
     setenv, delenv = monkeypatch.setenv, monkeypatch.delenv
 
     def _setenv(name, value, *a, **k):
@@ -74,4 +75,9 @@ def _dgs_tuning_follows_env(monkeypatch):
     monkeypatch.setenv, monkeypatch.delenv = _setenv, _delenv
     yield
     monkeypatch.undo()
+    # (a test that sets them past monkeypatch - the seeded fuzz slice does for each of its cases, and how many it gets through in its time
+    # decides what the last one leaves - does not hand them on to the next)
+    for k in [k for k in os.environ if k.startswith('DGS_') and k not in before]:
+        del os.environ[k]
+    os.environ.update(before)
     _capi.reload_tuning()
