@@ -203,7 +203,7 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const char *__restrict__ a
       for (int kk = 0; kk < 2; kk++) {
         const int64_t k = blk * 128 + kk * 64;
         const bool on = k + at < kbytes;  // (rows are multiples of 16 bytes)
-        y[s].u[kk] = on ? __builtin_nontemporal_load((const dgs_u4 *)(pb + k)) : zero;
+        y[s].u[kk] = on ? *(const dgs_u4 *)(pb + k) : zero;
 #pragma unroll
         for (int i = 0; i < FM; i++) x[s][i].u[kk] = on ? *(const dgs_u4 *)(pa[i] + k) : zero;
       }

@@ -185,8 +185,8 @@ __global__ __launch_bounds__(512) void gated_few_kernel(const char *__restrict__
       for (int kk = 0; kk < 2; kk++) {
         const int64_t k = k0 + (int64_t)s * kW * 128 + kk * 64;
         const bool on = k + (lane >> 4) * 16 < kbytes;
-        w[s][kk][0].u = on ? __builtin_nontemporal_load((const dgs_u4 *)(pg + k)) : zero;
-        w[s][kk][1].u = on ? __builtin_nontemporal_load((const dgs_u4 *)(pu + k)) : zero;
+        w[s][kk][0].u = on ? *(const dgs_u4 *)(pg + k) : zero;
+        w[s][kk][1].u = on ? *(const dgs_u4 *)(pu + k) : zero;
 #pragma unroll
         for (int i = 0; i < FM; i++) a[s][kk][i].u = on ? *(const dgs_u4 *)(px[i] + k) : zero;
       }
