@@ -177,9 +177,12 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const char *__restrict__ a
                                                       const Scales sc, T *__restrict__ out) {
   constexpr int kW = 8;
   __shared__ float sum[kW][16 * FM][17];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, at = (lane >> 4) * 16;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, n = n0 + r < N ? n0 + r : N - 1;
-  const char *pb = b + n * ldb + at;
+  __shared__ __align__(16) char turned[kW][16 * kStepBytes];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, at = (lane >> 4) * 16, piece = (lane & 7) * 16;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const char *pb[2];  // rows 0 - 7 and 8 - 15
+#pragma unroll
+  for (int q = 0; q < 2; q++) pb[q] = b + (n0 + 8 * q + (lane >> 3) < N ? n0 + 8 * q + (lane >> 3) : N - 1) * ldb + piece;
   const float *sb = sc.b + n0 / 128 * sc.blocks;
   const char *pa[FM];
   const float *sa[FM];
@@ -194,7 +197,8 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const char *__restrict__ a
   const dgs_u4 zero = {0u, 0u, 0u, 0u};
   constexpr int U = FM == 4 ? 2 : 4;  // blocks in flight
   for (int64_t k0 = wave; k0 < sc.blocks; k0 += kW * U) {
-    Slice8 y[U], x[U][FM];
+    Lines y[U];
+    Slice8 x[U][FM];
     float f[U][FM];
 #pragma unroll
     for (int s = 0; s < U; s++) {
@@ -203,7 +207,7 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const char *__restrict__ a
       for (int kk = 0; kk < 2; kk++) {
         const int64_t k = blk * 128 + kk * 64;
         const bool on = k + at < kbytes;  // (rows are multiples of 16 bytes)
-        y[s].u[kk] = on ? *(const dgs_u4 *)(pb + k) : zero;
+        y[s].u[kk] = blk * 128 + piece < kbytes ? *(const dgs_u4 *)(pb[kk] + blk * 128) : zero;
 #pragma unroll
         for (int i = 0; i < FM; i++) x[s][i].u[kk] = on ? *(const dgs_u4 *)(pa[i] + k) : zero;
       }
@@ -212,15 +216,19 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const char *__restrict__ a
       for (int i = 0; i < FM; i++) f[s][i] = blk < sc.blocks ? sa[i][blk] * t : 0.0f;
     }
 #pragma unroll
-    for (int s = 0; s < U; s++)
+    for (int s = 0; s < U; s++) {
+      Slice t[2];
+      turn(turned[wave], lane, y[s], t);
+      const Slice8 v = {.u = {t[0].u, t[1].u}};
 #pragma unroll
       for (int i = 0; i < FM; i++) {
-        const f32x4 part = block_product<T>(y[s], x[s][i]);
+        const f32x4 part = block_product<T>(v, x[s][i]);
         if (k0 + s * kW < sc.blocks) {
 #pragma unroll
           for (int k = 0; k < 4; k++) acc[i][k] = __builtin_fmaf(part[k], f[s][i], acc[i][k]);
         }
       }
+    }
   }
 #pragma unroll
   for (int i = 0; i < FM; i++)

@@ -159,16 +159,22 @@ __global__ __launch_bounds__(kBlock) void gated_split_kernel(int64_t M, int G, c
 // Few rows (<= 16 FM): 8 waves share the K of 16 columns of Wg and of Wu, whose rows go from memory to the registers of the matrix
 // instructions (128 bytes of each of 16 rows a wave at a time); x comes out of L2.  The waves' sums meet in LDS.
 template <typename T, int FM, int ACT>
-__global__ __launch_bounds__(512) void gated_few_kernel(const char *__restrict__ x, int64_t ldx, const char *__restrict__ wg, const char *__restrict__ wu, int64_t ldw,
+__global__ __launch_bounds__(512, sizeof(T) == 2 && FM < 4 ? 4 : 2) void gated_few_kernel(const char *__restrict__ x, int64_t ldx, const char *__restrict__ wg, const char *__restrict__ wu, int64_t ldw,
                                                         int M, int64_t F, int64_t kbytes, T *__restrict__ h,
                                                         float *__restrict__ pre) {
   constexpr int kW = 8;
   __shared__ float sum[kW][2][16 * FM][17];
+  __shared__ __align__(16) char turned[kW][2][16 * kStepBytes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int r = lane & 15;
-  const int64_t n = n0 + r < F ? n0 + r : F - 1;
-  const char *pg = wg + n * ldw + (lane >> 4) * 16, *pu = wu + n * ldw + (lane >> 4) * 16;
+  const int r = lane & 15, piece = (lane & 7) * 16;
+  const char *pg[2], *pu[2];  // rows 0 - 7 and 8 - 15
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    const int64_t n = n0 + 8 * q + (lane >> 3) < F ? n0 + 8 * q + (lane >> 3) : F - 1;
+    pg[q] = wg + n * ldw + piece;
+    pu[q] = wu + n * ldw + piece;
+  }
   const char *px[FM];
 #pragma unroll
   for (int i = 0; i < FM; i++) px[i] = x + (int64_t)(16 * i + r < M ? 16 * i + r : M - 1) * ldx + (lane >> 4) * 16;
@@ -178,22 +184,36 @@ __global__ __launch_bounds__(512) void gated_few_kernel(const char *__restrict__
   const dgs_u4 zero = {0u, 0u, 0u, 0u};
   constexpr int U = FM == 1 ? 4 : 2;  // 128-byte steps in flight
   for (int64_t k0 = wave * 128; k0 < kbytes; k0 += kW * 128 * U) {
-    Slice w[U][2][2], a[U][2][FM];  // (the rows of Wg and of Wu)
+    Lines w[U][2];  // (of Wg and of Wu)
+    Slice a[U][2][FM];
 #pragma unroll
-    for (int s = 0; s < U; s++)
+    for (int s = 0; s < U; s++) {
+      const int64_t k = k0 + (int64_t)s * kW * 128;
+      const bool there = k + piece < kbytes;
 #pragma unroll
-      for (int kk = 0; kk < 2; kk++) {
-        const int64_t k = k0 + (int64_t)s * kW * 128 + kk * 64;
-        const bool on = k + (lane >> 4) * 16 < kbytes;
-        w[s][kk][0].u = on ? *(const dgs_u4 *)(pg + k) : zero;
-        w[s][kk][1].u = on ? *(const dgs_u4 *)(pu + k) : zero;
-#pragma unroll
-        for (int i = 0; i < FM; i++) a[s][kk][i].u = on ? *(const dgs_u4 *)(px[i] + k) : zero;
+      for (int q = 0; q < 2; q++) {
+        w[s][0].u[q] = there ? *(const dgs_u4 *)(pg[q] + k) : zero;
+        w[s][1].u[q] = there ? *(const dgs_u4 *)(pu[q] + k) : zero;
       }
 #pragma unroll
-    for (int s = 0; s < U; s++)
+      for (int kk = 0; kk < 2; kk++) {
+        const bool on = k + kk * 64 + (lane >> 4) * 16 < kbytes;
 #pragma unroll
-      for (int kk = 0; kk < 2; kk++) multiply<T>(a[s][kk], w[s][kk], acc);
+        for (int i = 0; i < FM; i++) a[s][kk][i].u = on ? *(const dgs_u4 *)(px[i] + k + kk * 64) : zero;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < U; s++) {
+      Slice v[2][2], b[2];  // [matrix][kk]
+      turn(turned[wave][0], lane, w[s][0], v[0]);
+      turn(turned[wave][1], lane, w[s][1], v[1]);
+#pragma unroll
+      for (int kk = 0; kk < 2; kk++) {
+        b[0] = v[0][kk];
+        b[1] = v[1][kk];
+        multiply<T>(a[s][kk], b, acc);
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < FM; i++)

@@ -441,6 +441,28 @@ struct Gemm3 : Shares<BM, BN, WM, WN, PAIR> {
   }
 };
 
+// ---- few rows of A: the rows of B on their way to a wave's matrix instructions ---------------------------------------------------------
+// A wave loads 16 rows x 128 bytes in two loads of 8 whole lines: neighbouring lanes take neighbouring 16 bytes (16 rows x 64 bytes a load, as the
+// instruction wants them, reads 45 MB at 4.6 TB/s, these at 5.7), and turns them by way of 2 KB of LDS of its own into the two slices.
+// Only this wave touches them, and a wave's LDS accesses are made in their order: no barrier, only the compiler is held.
+struct Lines {
+  dgs_u4 u[2];
+};
+__device__ __forceinline__ void turn(char *lds, int lane, const Lines &x, Slice (&s)[2]) {
+  using L = Tile<bf16, 16, false>;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int row = 8 * h + (lane >> 3);
+    *reinterpret_cast<dgs_u4 *>(lds + row * kStepBytes + L::mix(row, lane & 7) * 16) = x.u[h];
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int kk = 0; kk < 2; kk++) L::read(lds, 0, kk, lane, s[kk]);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // four neighbouring columns of a row; `vec`: the row's stride and base allow one store
 template <typename T>
 __device__ __forceinline__ void store4(T *p, const f32x4 &v, int64_t left, bool vec) {
