@@ -7,7 +7,7 @@
 // needs one scale of a for each 16 rows; a wave's columns lie within one block of 128, so the scale of b is the wave's.
 // Bound: many rows: the matrix cores, with four multiply-adds a lane beside each instruction; few rows: the bytes of b (fp8_few_kernel).
 // Measured: 4095 x 11000 x 4096, bf16 out: 196 - 215 us (1.7 - 1.9 PFLOP/s; a large product without block scales, the library's: 2.7);
-// 5 x 4096 x 11008: 13.3 us a call (45 MB: 3.4 TB/s).
+// 5 x 4096 x 11008: 10.0 us (45 MB: 4.5 TB/s), 1 x 32000 x 4096: 23.4 (5.6).
 #include "gemm_core.h"
 
 namespace dgs {
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(64 * WM *WN) void fp8_kernel(const GemmArgs g, cons
   }
 }
 
-// Few rows (<= 16 FM): 8 waves share the blocks of K of 16 columns; b goes from memory to the matrix instructions' registers.
+// Few rows (<= 16 FM): 8 waves share the blocks of K of 16 columns; b goes from memory, whole lines at a time (`turn`), to the matrix instructions.
 template <typename T, int FM>
 __global__ __launch_bounds__(512) void fp8_few_kernel(const char *__restrict__ a, int64_t lda, const char *__restrict__ b, int64_t ldb, int M, int64_t N, int64_t kbytes,
                                                       const Scales sc, T *__restrict__ out) {
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const char *__restrict__ a
     acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
   const dgs_u4 zero = {0u, 0u, 0u, 0u};
-  constexpr int U = FM == 4 ? 2 : 4;  // blocks in flight
+  constexpr int U = FM == 1 ? 2 : 1;  // blocks in flight (few: registers for more workgroups on a CU instead; 4 of them: 1 x 32000 x 4096 25.5 us, 2: 23.4)
   for (int64_t k0 = wave; k0 < sc.blocks; k0 += kW * U) {
     Lines y[U];
     Slice8 x[U][FM];
@@ -322,7 +322,10 @@ static int quantize(int64_t rows, int64_t cols, const void *x, int64_t ld, int b
   return check_launch();
 }
 
-constexpr int64_t kFewRows8 = 64;
+// Products that take fp8_few_kernel: beyond 16 rows its reads of a out of L2 for every 16 columns outweigh the 64-row tiles' waste, but for small b
+// (few and tiles: 32 x 2048 x 2048 4.9 and 5.9 us, 32 x 4096 x 4096 8.1 and 8.4;  17 x 4096 x 11008 11.2 and 13.2, 32 x 4096 x 11008 15.2 and 13.9, 32 x 32000 x 4096 51
+// and 30).
+static bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= 16 || (M <= 32 && N * K <= (1 << 24)); }
 
 struct Layout8 {
   bool pad;
@@ -339,7 +342,7 @@ static Layout8 layout8(int64_t M, int64_t N, int64_t K, bool wide) {  // wide: t
   L.a = take(L.pad ? (size_t)M * L.ldk : 0);
   L.b = take(L.pad ? (size_t)N * L.ldk : 0);
   L.plan = tile_plan(M, N, (K + 127) / 128, 1, false, wide, true);
-  L.partial = take(M > kFewRows8 && L.plan.splits > 1 ? (size_t)L.plan.splits * M * N * 4 : 0);
+  L.partial = take(!few_rows(M, N, K) && L.plan.splits > 1 ? (size_t)L.plan.splits * M * N * 4 : 0);
   L.total = at;
   return L;
 }
@@ -357,12 +360,11 @@ static int matmul8(int64_t M, int64_t N, int64_t K, const void *a, int64_t lda, 
     lda = ldb = L.ldk;
   }
   const Scales sc = {sa, sb, (K + 127) / 128};
-  if (M <= kFewRows8) {
+  if (few_rows(M, N, K)) {
     if (!grid_ok((N + 15) / 16, 512)) return DGS_ERANGE;
     const dim3 grid((unsigned)((N + 15) / 16));
     if (M <= 16) hipLaunchKernelGGL((fp8_few_kernel<T, 1>), grid, dim3(512), 0, st, ap, lda, bp, ldb, (int)M, N, L.ldk, sc, out);
-    else if (M <= 32) hipLaunchKernelGGL((fp8_few_kernel<T, 2>), grid, dim3(512), 0, st, ap, lda, bp, ldb, (int)M, N, L.ldk, sc, out);
-    else hipLaunchKernelGGL((fp8_few_kernel<T, 4>), grid, dim3(512), 0, st, ap, lda, bp, ldb, (int)M, N, L.ldk, sc, out);
+    else hipLaunchKernelGGL((fp8_few_kernel<T, 2>), grid, dim3(512), 0, st, ap, lda, bp, ldb, (int)M, N, L.ldk, sc, out);
     return check_launch();
   }
   const TilePlan &p = L.plan;

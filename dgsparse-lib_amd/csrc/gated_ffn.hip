@@ -11,7 +11,6 @@
 // (gated_few_kernel).  Sums are held in 32 bits.
 // Measured, forward and backward: 4096 x 4096 x 11008 bf16 2.04 ms (1.09 PFLOP/s; the library's plain products of this shape run at 0.86, of
 // 8192^3 at 1.2 - 1.3);  169343 x 128 x 512 fp32 1.18 ms (150 TFLOP/s with the products made again; the library's 32-bit products: 153).
-// Few rows: 3 x 2048 x 5504 fp16 14.9 us a call (45 MB: 3.0 TB/s).
 #include "gemm_core.h"
 
 namespace dgs {
@@ -156,10 +155,11 @@ __global__ __launch_bounds__(kBlock) void gated_split_kernel(int64_t M, int G, c
   }
 }
 
-// Few rows (<= 16 FM): 8 waves share the K of 16 columns of Wg and of Wu, whose rows go from memory to the registers of the matrix
-// instructions (128 bytes of each of 16 rows a wave at a time); x comes out of L2.  The waves' sums meet in LDS.
+// Few rows (<= 16 FM): 8 waves share the K of 16 columns of Wg and of Wu, whose rows go from memory, whole lines at a time (`turn`), to the
+// matrix instructions; x comes out of L2.  The waves' sums meet in LDS.  3 x 2048 x 5504 fp16: 9.4 us (45 MB: 4.8 TB/s; a plain read of as much, in
+// order: 7.1), 1 x 4096 x 11008 bf16: 31.6 us (5.7 TB/s).
 template <typename T, int FM, int ACT>
-__global__ __launch_bounds__(512, sizeof(T) == 2 && FM < 4 ? 4 : 2) void gated_few_kernel(const char *__restrict__ x, int64_t ldx, const char *__restrict__ wg, const char *__restrict__ wu, int64_t ldw,
+__global__ __launch_bounds__(512, sizeof(T) == 2 && FM < 3 ? 4 : 2) void gated_few_kernel(const char *__restrict__ x, int64_t ldx, const char *__restrict__ wg, const char *__restrict__ wu, int64_t ldw,
                                                         int M, int64_t F, int64_t kbytes, T *__restrict__ h,
                                                         float *__restrict__ pre) {
   constexpr int kW = 8;
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(512, sizeof(T) == 2 && FM < 4 ? 4 : 2) void gated_f
 #pragma unroll
   for (int i = 0; i < FM; i++) acc[i][0] = acc[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const dgs_u4 zero = {0u, 0u, 0u, 0u};
-  constexpr int U = FM == 1 ? 4 : 2;  // 128-byte steps in flight
+  constexpr int U = FM == 1 ? 4 : 1;  // 128-byte steps in flight (few: registers for more workgroups on a CU instead)
   for (int64_t k0 = wave * 128; k0 < kbytes; k0 += kW * 128 * U) {
     Lines w[U][2];  // (of Wg and of Wu)
     Slice a[U][2][FM];
@@ -378,7 +378,13 @@ static int launch_product(GemmArgs g, PlainOut o, const TilePlan &p, float *part
   return DGS_OK;
 }
 
-constexpr int64_t kFewRows = 64;
+// Products that take gated_few_kernel.  Beyond 48 rows its reads of x out of L2 for every 16 columns cost more than the 64-row tiles' waste, if
+// those fill the card.  Few and tiles, us: 2048 x 5504 fp16: 32 rows 13.9 and 18.5, 48 rows 17.7 and 18.6, 64 rows 22.1 and 18.8;  64 x 4096 x 4096 bf16 (128
+// tiles) 20.9 and 33.7;  1024 x 4096 fp32: 48 rows 15.1 and 22.9, 64 rows 19.3 and 23.0.
+template <typename T>
+static bool few_rows(int64_t rows, int64_t F) {
+  return rows <= 48 || (rows <= 64 && (sizeof(T) == 4 || (F + 31) / 32 < cu_count() * 5 / 8));
+}
 
 template <typename T, int ACT>
 static int ffn_fwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, void *h, float *pre, char *ws, hipStream_t st) {
@@ -386,13 +392,14 @@ static int ffn_fwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ld
   Operands<T> op;
   const int rc = operands<T>(rows, D, F, x, ldx, wg, wu, ldw, ws, L, st, op);
   if (rc != DGS_OK) return rc;
-  if (rows <= kFewRows) {
+  if (few_rows<T>(rows, F)) {
     if (!grid_ok((F + 15) / 16, 512)) return DGS_ERANGE;
     const dim3 grid((unsigned)((F + 15) / 16));
     const int64_t kb = (int64_t)(L.pad ? L.ldx : D) * (int64_t)sizeof(T), lx = op.ldx * (int64_t)sizeof(T), lw = op.ldw * (int64_t)sizeof(T);
 #define DGS_FEW(FM_) hipLaunchKernelGGL((gated_few_kernel<T, FM_, ACT>), grid, dim3(512), 0, st, op.x, lx, op.wg, op.wu, lw, (int)rows, F, kb, (T *)h, pre)
     if (rows <= 16) DGS_FEW(1);
     else if (rows <= 32) DGS_FEW(2);
+    else if (rows <= 48) DGS_FEW(3);
     else DGS_FEW(4);
 #undef DGS_FEW
     return check_launch();
