@@ -60,8 +60,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activat
     needs the projections: ``recompute=False`` keeps both in 32 bits, ``True`` makes them again, ``None`` keeps them where that is faster
     and takes no more than 1 GiB.  Both ways give results within the rounding of the other (the same bits from 65 rows on).
 
-    In float32 a value takes part as the sum of three of 16 bits (products as close as ones rounded to 32 bits): an infinity in ``x`` or a
-    weight gives NaN, in the rows that it reaches."""
+    In float32 a value takes part as the sum of three of 16 bits (products as close as ones rounded to 32 bits): beyond 64 rows
+    an infinity in ``x`` or a weight (or a magnitude above 3.38e38) gives NaN, in the rows that it reaches."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f'dgsparse: activation must be one of {sorted(_ACTIVATIONS)}, not {activation!r}')
     return _gated_ffn(x, w_gate, w_up, _ACTIVATIONS[activation], -1 if recompute is None else int(not recompute))

@@ -484,6 +484,34 @@ def test_matmul_fp8_layouts():
     assert bad[2, 1].isnan().all() and torch.equal(bad[:2], out[:2]) and torch.equal(bad[3:], out[3:])
 
 
+# ---- where few rows end -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('t', TYPES, ids=ids_of)
+@pytest.mark.parametrize('T,D,F', [(33, 72, 40), (48, 264, 130), (49, 40, 64), (64, 136, 5119), (49, 24, 5200), (64, 40, 5200)])
+def test_gated_ffn_on_either_side_of_few_rows(T, D, F, t):
+    check_ffn(rand(T, D, t=t, seed=1), rand(F, D, t=t, seed=2, scale=D ** -0.5), rand(F, D, t=t, seed=3, scale=D ** -0.5), 'gelu')
+
+
+@pytest.mark.parametrize('t', TYPES, ids=ids_of)
+@pytest.mark.parametrize('M,N,K', [(16, 4100, 4200), (17, 4100, 4200), (32, 4096, 4096), (32, 4112, 4096), (33, 40, 300), (17, 1, 4096)])
+def test_matmul_fp8_on_either_side_of_few_rows(M, N, K, t):
+    import dgsparse
+    a, sa = dgsparse.quantize_fp8(rand(M, K, t=torch.float32, seed=1))
+    b, sb = dgsparse.quantize_fp8(rand(N, K, t=torch.float32, seed=2), 128)
+    check_mm8(a, sa, b, sb, t)
+
+
+def test_gated_ffn_rows_of_infinities_in_the_tiles():
+    """32 bits beyond the few rows: an infinity is a NaN in the rows that it reaches, and in no other."""
+    import dgsparse
+    x, wg, wu = rand(200, 40, t=torch.float32, seed=1), rand(70, 40, t=torch.float32, seed=2, scale=0.2), rand(70, 40, t=torch.float32, seed=3, scale=0.2)
+    bad = x.clone()
+    bad[[0, 63, 128, 199], [0, 3, 39, 17]] = torch.tensor([math.inf, -math.inf, math.inf, -math.inf], device='cuda')
+    h = dgsparse.gated_ffn(bad, wg, wu, 'gelu')
+    good = torch.ones(200, dtype=torch.bool, device='cuda')
+    good[[0, 63, 128, 199]] = False
+    assert h[~good].isnan().all() and torch.equal(h[good], dgsparse.gated_ffn(x, wg, wu, 'gelu')[good])
+
+
 # ---- together, streams, graphs ----------------------------------------------------------------------------------------------
 def chain(ids, table, norm, wg, wu, aq, asc):
     """lookup -> residual norm -> gated product -> 8-bit projection"""
