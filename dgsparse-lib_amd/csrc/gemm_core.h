@@ -289,19 +289,25 @@ __device__ __forceinline__ void gemm_loop(const GemmArgs &g, int m0, int n0, int
 //
 // What is left of a value is one instruction, the dot product of its pair's parts with (-1, 0) or (0, -1) added to it: exact, like the
 // subtraction it stands for, without the part widened to 32 bits first (7 instructions a pair for the three parts, not 11).  The constants
-// are kept in registers: as inline constants these instructions take them for both halves.
+// are kept in registers: as inline constants these instructions take them for both halves.  The pair's other value enters such a product as 0
+// times it, which an infinity or a NaN makes a NaN: right where the two lie in one row (K-inner: the row has the value either way), wrong where
+// they lie in two (K-outer, ALONE: dW's row of a good gradient beside a bad one).  There each value is widened and subtracted by itself.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 struct Minus {  // (-1, 0) and (0, -1) in bf16
   uint32_t lo = 0x0000bf80u, hi = 0xbf800000u;
   __device__ __forceinline__ Minus() { asm volatile("" : "+s"(lo), "+s"(hi)); }
 };
+template <bool ALONE>
 __device__ __forceinline__ void split3(f32x2 r, const Minus &minus, uint32_t (&part)[3]) {
 #pragma unroll
   for (int q = 0; q < 3; q++) {
     const bf16x2 h = __builtin_convertvector(r, bf16x2);
     part[q] = __builtin_bit_cast(uint32_t, h);
-    if (q < 2) {
+    if (q < 2 && ALONE) {
+      r[0] -= (float)h[0];
+      r[1] -= (float)h[1];
+    } else if (q < 2) {
       r[0] = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, minus.lo), r[0], false);
       r[1] = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, minus.hi), r[1], false);
     }
@@ -328,7 +334,7 @@ struct Planes {
     const int row = id / kPieces, piece = id % kPieces;
     uint32_t p[2][3];
 #pragma unroll
-    for (int h = 0; h < 2; h++) split3(f32x2{x[2 * h], x[2 * h + 1]}, minus, p[h]);
+    for (int h = 0; h < 2; h++) split3<KO>(f32x2{x[2 * h], x[2 * h + 1]}, minus, p[h]);
     char *at = lds + row * (KO ? 2 * R : 64) + mix(row, piece / 2) * 16 + piece % 2 * 8;
 #pragma unroll
     for (int q = 0; q < 3; q++) *reinterpret_cast<dgs_u2 *>(at + q * kPlane) = dgs_u2{p[0][q], p[1][q]};
