@@ -5,6 +5,8 @@
 //       that forward and backward see the same values)
 //   y = s r w,  r = 1 / sqrt(mean(s^2) + eps)
 //   dx = dresidual = r (w dy) - s r^3 mean(s w dy) + ds ;  dw = sum over rows of dy s r
+//       taken as r (w dy - (s r) (r mean(s w dy))) + ds: every factor is an ordinary number where s and its squares' sum are, while r^3 by itself
+//       leaves the range of 32 bits for rows beyond 1e13 or (with an eps next to nothing) below 1e-13
 //
 // Bound: HBM.  Forward reads 2 rows and writes 2, backward reads 3 and writes 1; a row is read once and stays in registers between its
 // reduction and its use (NV 16-byte vectors per lane).  Row statistics and dw are sums in 32 bits.
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(kBlock) void rms_norm_bwd_kernel(int64_t rows, int 
     sq = group_sum<G>(sq, red[turn][0]);  // (two sets of LDS slots: a row's sums are read while the next row's are written)
     dot = group_sum<G>(dot, red[turn][1]);
     const float r = 1.0f / sqrtf(sq / (float)D + eps);
-    const float k3 = r * r * r * (dot / (float)D);
+    const float m = r * (dot / (float)D);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
       const int c = (lane + j * G) * V;
@@ -189,8 +191,9 @@ __global__ __launch_bounds__(kBlock) void rms_norm_bwd_kernel(int64_t rows, int 
       }
 #pragma unroll
       for (int k = 0; k < V; k++) {
-        o[k] += r * (g[j][k] * gy[j][k]) - sv[j][k] * k3;
-        acc[j][k] = __builtin_fmaf(gy[j][k], sv[j][k] * r, acc[j][k]);
+        const float n = sv[j][k] * r;
+        o[k] = __builtin_fmaf(r, __builtin_fmaf(-n, m, g[j][k] * gy[j][k]), o[k]);
+        acc[j][k] = __builtin_fmaf(gy[j][k], n, acc[j][k]);
       }
       store_row<T, VECTOR>(dx + at, c, D, o);
     }
@@ -236,11 +239,11 @@ __global__ __launch_bounds__(kBlock) void rms_norm_bwd_long_kernel(int D, const 
   sq = group_sum<256>(sq, red[0]);
   dot = group_sum<256>(dot, red[1]);
   const float r = 1.0f / sqrtf(sq / (float)D + eps);
-  const float k3 = r * r * r * (dot / (float)D);
+  const float m = r * (dot / (float)D);
   if (rstd && threadIdx.x == 0) rstd[row] = r;
   for (int c = threadIdx.x; c < D; c += kBlock) {
-    const float o = (DS ? to_f32(ds[at + c]) : 0.0f) + r * (to_f32(w[c]) * to_f32(dy[at + c])) - to_f32(s[at + c]) * k3;
-    dx[at + c] = from_f32<T>(o);
+    const float n = to_f32(s[at + c]) * r, o = DS ? to_f32(ds[at + c]) : 0.0f;
+    dx[at + c] = from_f32<T>(__builtin_fmaf(r, __builtin_fmaf(-n, m, to_f32(w[c]) * to_f32(dy[at + c])), o));
   }
 }
 template <typename T>

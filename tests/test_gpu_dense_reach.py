@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_dense import TYPES, ids_of, rand
+from test_gpu_dense import E32, TYPES, U, ids_of, norm_want, rand, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,24 @@ def test_gated_ffn_a_closed_unit_stays_in_its_column():
     open_ = torch.ones(D, dtype=torch.bool, device='cuda')
     open_[[6, 11, 23]] = False
     assert dx[:, ~open_].isnan().all() and dx[:, open_].isfinite().all()
+
+
+# ---- magnitudes ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('t', [torch.float32, torch.bfloat16], ids=ids_of)
+@pytest.mark.parametrize('scale,eps', [(1e13, 1e-6), (1e15, 1e-6), (1e16, 1e-6), (1e-12, 0.0), (1e-14, 0.0), (1e-16, 0.0), (1e-14, 1e-30)])
+@pytest.mark.parametrize('rows,D', [(5, 64), (9, 1000), (3, 4096), (2, 16390)])
+def test_rms_norm_gradient_at_any_magnitude(rows, D, scale, eps, t):
+    """s, its squares' sum and the gradient are all within the type's range (s^2 sums to at most 2e4 * 1e32, at least 64 * 1e-32)."""
+    import dgsparse
+    x = rand(rows, D, t=t, seed=1, scale=scale).requires_grad_()
+    w = (1 + rand(D, t=torch.float32, seed=3, scale=0.1)).to(t).requires_grad_()
+    dy, ds = rand(rows, D, t=t, seed=4), rand(rows, D, t=t, seed=5, scale=1 / scale)
+    y, s = dgsparse.add_rms_norm(x, torch.zeros_like(x), w, eps)
+    assert torch.equal(s, x)
+    dx, dw = torch.autograd.grad((y, s), (x, w), (dy, ds))
+    eps = torch.tensor(eps, dtype=torch.float32).double().item()  # (the entry takes a float)
+    wy, wdx, mag, wdw, wmag = norm_want(s.detach(), w.detach(), eps, dy, ds)
+    n = D + 16  # as at ordinary magnitudes: a mean over D, its root, some products
+    within(y, wy, wy.abs() * (U(t) + n * E32) + tiny(t), 'y')
+    within(dx, wdx, wdx.abs() * U(t) + 2 * n * E32 * mag + tiny(t), 'dx')
+    within(dw, wdw, wdw.abs() * U(t) + (n + rows) * E32 * wmag + tiny(t), 'dw')
