@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <initializer_list>
 #include <tuple>
 
 #include "dgsparse_hip.h"
@@ -53,6 +54,11 @@ Tensor rows_of(const Tensor &t, int64_t &ld) {
 // These nodes are differentiable once: with create_graph the second gradient would silently miss their part.
 void once(const char *what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "dgsparse: ", what, " is differentiable once (its backward pass has no gradient of its own: no create_graph)");
+}
+// Nor have they a forward-mode derivative: where no gradient is recorded, a tangent would be dropped without a word, which stands for 0.
+void no_tangent(const char *what, std::initializer_list<const Tensor *> inputs) {
+  for (const Tensor *t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "dgsparse: ", what, " has no forward-mode derivative");
 }
 
 // ---- embedding -------------------------------------------------------------------------------------------------------------
@@ -107,6 +113,7 @@ struct Embedding : public torch::autograd::Function<Embedding> {
 };
 Tensor embedding_op(Tensor ids, Tensor table, double scale, int64_t padding_idx) {
   TORCH_CHECK(padding_idx < table.size(0), "dgsparse: padding_idx ", padding_idx, " is not a row of the table");
+  no_tangent("embedding", {&table});
   if (!(at::GradMode::is_enabled() && table.requires_grad())) return embedding_fwd(ids, table, scale);
   return Embedding::apply(table, ids, scale, padding_idx);
 }
@@ -191,10 +198,12 @@ struct AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
   }
 };
 Tensor rms_norm_op(Tensor x, Tensor weight, double eps) {
+  no_tangent("rms_norm", {&x, &weight});
   if (!(at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))) return norm_fwd(x, Tensor(), weight, eps, false).y;
   return RmsNorm::apply(x, weight, eps);
 }
 std::tuple<Tensor, Tensor> add_rms_norm_op(Tensor x, Tensor residual, Tensor weight, double eps) {
+  no_tangent("add_rms_norm", {&x, &residual, &weight});
   if (!(at::GradMode::is_enabled() && (x.requires_grad() || residual.requires_grad() || weight.requires_grad()))) {
     NormOut o = norm_fwd(x, residual, weight, eps, false);
     return {o.y, o.s};
@@ -312,6 +321,7 @@ struct GatedFfn : public torch::autograd::Function<GatedFfn> {
 };
 Tensor gated_ffn_op(Tensor x, Tensor wg, Tensor wu, int64_t activation, int64_t keep) {
   ffn_check(x, wg, wu, activation);
+  no_tangent("gated_ffn", {&x, &wg, &wu});
   if (!(at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad()))) return ffn_fwd(x, wg, wu, activation);
   return GatedFfn::apply(x, wg, wu, activation, keep);
 }

@@ -3,8 +3,8 @@ hand-written gfx950 kernels (csrc/embedding.hip, rms_norm.hip, gated_ffn.hip, fp
 
 All of them take float32, float16 and bfloat16 tensors on the GPU (one type a call), run on the current stream of the tensors' device,
 never synchronise, and may be captured into a graph.  Sums and row statistics are held in 32 bits; a result is rounded to its type once.
-Where a gradient is offered it is that of the formula given, once (no gradient of a gradient).  New: the reference's layers call torch
-for all of this (dgsparse/nn/gcnconv.py:10-35, ginconv.py:9-70)."""
+Where a gradient is offered it is that of the formula given, once (no gradient of a gradient, and no forward-mode derivative: both
+raise).  New: the reference's layers call torch for all of this (dgsparse/nn/gcnconv.py:10-35, ginconv.py:9-70)."""
 from typing import Optional, Tuple
 
 import torch

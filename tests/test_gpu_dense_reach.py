@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from test_gpu_dense import E32, TYPES, U, ids_of, norm_want, rand, tiny, within
 
@@ -70,3 +71,26 @@ def test_rms_norm_gradient_at_any_magnitude(rows, D, scale, eps, t):
     within(y, wy, wy.abs() * (U(t) + n * E32) + tiny(t), 'y')
     within(dx, wdx, wdx.abs() * U(t) + 2 * n * E32 * mag + tiny(t), 'dx')
     within(dw, wdw, wdw.abs() * U(t) + (n + rows) * E32 * wmag + tiny(t), 'dw')
+
+
+# ---- forward-mode derivatives ---------------------------------------------------------------------------------------------------
+def test_forward_mode_derivatives_are_refused():
+    """They have none: a tangent that came back empty would stand for 0."""
+    import dgsparse
+    x, w, m = rand(6, 16, t=torch.float32, seed=1), rand(16, t=torch.float32, seed=2), rand(8, 16, t=torch.float32, seed=3)
+    ids = torch.arange(4, device='cuda')
+    calls = [(x, lambda a: dgsparse.embedding(ids, a)), (x, lambda a: dgsparse.rms_norm(a, w)), (w, lambda a: dgsparse.rms_norm(x, a)),
+             (x, lambda a: dgsparse.add_rms_norm(a, x, w)), (x, lambda a: dgsparse.add_rms_norm(x, a, w)), (w, lambda a: dgsparse.add_rms_norm(x, x, a)),
+             (x, lambda a: dgsparse.gated_ffn(a, m, m)), (m, lambda a: dgsparse.gated_ffn(x, a, m)), (m, lambda a: dgsparse.gated_ffn(x, m, a))]
+    for i, (primal, f) in enumerate(calls):
+        for needs_grad in (False, True):
+            with fwad.dual_level():
+                dual = fwad.make_dual(primal.clone().requires_grad_(needs_grad), torch.ones_like(primal))
+                with pytest.raises(RuntimeError, match='forward-mode'):
+                    f(dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match='forward-mode'):
+                    f(dual)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (primal,), (torch.ones_like(primal),))
+        with fwad.dual_level():  # a dual level alone is no reason
+            f(primal)
