@@ -9,6 +9,8 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <climits>
 #include <initializer_list>
 #include <tuple>
 
@@ -217,11 +219,13 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8_op(Tensor x, Tensor residual
 }
 
 // ---- gated feed-forward ----------------------------------------------------------------------------------------------------
-// rows whose base and distance suit 16-byte accesses: t as it is, or a contiguous copy
+// rows whose base and distance suit 16-byte accesses, and whose distance the entries take (256 rows within 32 bits of bytes): t as it is, or a
+// contiguous copy (of [batch, length, features][:, -1], say: few rows, far apart)
 Tensor rows16_of(const Tensor &t, int64_t &ld) {
   Tensor r = rows_of(t, ld);
-  const int64_t v = 16 / (int64_t)r.element_size();
-  if (r.size(-1) % v == 0 && (ld % v || reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 || ld < r.size(-1))) {
+  const int64_t size = (int64_t)r.element_size(), v = 16 / size;
+  const bool far = ld > std::max<int64_t>(INT32_MAX / 256 / size - 64, r.size(-1));
+  if (far || (r.size(-1) % v == 0 && (ld % v || reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 || ld < r.size(-1)))) {
     r = r.clone(at::MemoryFormat::Contiguous);
     ld = r.size(-1);
   }

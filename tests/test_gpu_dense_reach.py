@@ -5,7 +5,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
-from test_gpu_dense import E32, TYPES, U, ids_of, norm_want, rand, tiny, within
+from test_gpu_dense import E32, TYPES, U, check_mm8, ids_of, norm_want, rand, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +94,32 @@ def test_forward_mode_derivatives_are_refused():
             torch.func.jvp(f, (primal,), (torch.ones_like(primal),))
         with fwad.dual_level():  # a dual level alone is no reason
             f(primal)
+
+
+# ---- rows far apart -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('t,L,D', [(torch.bfloat16, 2049, 2048), (torch.float32, 2049, 1024), (torch.float32, 2100, 1001)], ids=str)
+def test_gated_ffn_of_every_sequence_s_last_token(t, L, D):
+    """[batch, length, features][:, -1]: rows further apart than a tile's 32-bit offsets reach."""
+    import dgsparse
+    x = rand(3, L, D, t=t, seed=1)[:, -1]
+    assert x.stride(0) * 256 * t.itemsize > 2 ** 31
+    leaves = [a.requires_grad_() for a in (rand(40, D, t=t, seed=2, scale=D ** -0.5), rand(40, D, t=t, seed=3, scale=D ** -0.5))]
+    dh = rand(3, 40, t=t, seed=4)
+    outs = []
+    for v in (x, x.contiguous()):
+        v = v.detach().requires_grad_()
+        h = dgsparse.gated_ffn(v, *leaves)
+        outs.append((h,) + torch.autograd.grad(h, [v] + leaves, dh))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('L,K', [(4097, 2048), (4400, 2000), (4300, 2001)])
+def test_matmul_fp8_of_every_sequence_s_last_token(L, K):
+    import dgsparse
+    a, sa = dgsparse.quantize_fp8(rand(3, L, K, t=torch.bfloat16, seed=1))
+    b, sb = dgsparse.quantize_fp8(rand(130, K, t=torch.float32, seed=2), 128)
+    a, sa = a[:, -1], sa[:, -1]
+    assert a.stride(0) * 256 > 2 ** 31
+    out = check_mm8(a, sa, b, sb, torch.bfloat16)
+    assert torch.equal(out, dgsparse.matmul_fp8(a.view(torch.uint8).contiguous().view(a.dtype), sa.contiguous(), b, sb, torch.bfloat16))
