@@ -294,9 +294,9 @@ __global__ __launch_bounds__(kBlock) void embedding_bwd_kernel(int64_t n, int64_
 // Border b between chunks b - 1 and b: the workgroups of the row that starts in chunk b - 1 and goes on in chunk b add up its partial
 // sums: the start's, then one of each chunk up to the last.  32 columns x 8 shares of the chunks; the shares' sums are joined in order.
 template <typename T, int V>  // V columns a lane: 4, or 1 where a row of partial sums is no multiple of 16 bytes
-__global__ __launch_bounds__(kBlock) void embedding_join_kernel(int64_t n, int64_t vocab, int D, int chunk, int64_t n_chunks, const uint32_t *__restrict__ skey,
+__global__ __launch_bounds__(kBlock) void embedding_join_kernel(int64_t first, int64_t vocab, int D, int chunk, int64_t n_chunks, const uint32_t *__restrict__ skey,
                                                                 float scale, const float *__restrict__ partial, T *__restrict__ dtable) {
-  const int64_t b = (int64_t)blockIdx.x + 1;
+  const int64_t b = first + blockIdx.x;
   const int64_t at = b * chunk;
   const uint32_t key = skey[at];
   const uint32_t prev = skey[at - 1], start = b > 1 ? skey[at - chunk - 1] : 0xffffffffu;
@@ -451,16 +451,18 @@ static int bwd(int64_t n, int64_t V, int64_t D, const uint32_t *key, const int *
   else
     hipLaunchKernelGGL((embedding_bwd_kernel<T, false>), grid, dim3(kBlock), 0, st, n, V, (int)D, G, chunk, n_chunks, (int)tiles, work, fill_rows, keep, key, pos, (const T *)dout, ldo, scale, (T *)dtable, partial);
   if (check_launch() != DGS_OK) return DGS_ELAUNCH;
-  if (n_chunks > 1) {
-    const int64_t cols = (D + 31) / 32;
+  const int64_t cols = (D + 31) / 32, most = 0xffffffffll / kBlock;  // (a launch holds 2^24 - 1 workgroups in a row)
+  for (int64_t first = 1; first < n_chunks; first += most) {
+    const unsigned borders = (unsigned)(n_chunks - first < most ? n_chunks - first : most);
     if (D % 4 == 0)
-      hipLaunchKernelGGL((embedding_join_kernel<T, 4>), dim3((unsigned)(n_chunks - 1), (unsigned)((cols + 3) / 4 < 16 ? (cols + 3) / 4 : 16)), dim3(kBlock), 0, st, n, V, (int)D, chunk,
-                         n_chunks, key, scale, partial, (T *)dtable);
+      hipLaunchKernelGGL((embedding_join_kernel<T, 4>), dim3(borders, (unsigned)((cols + 3) / 4 < 16 ? (cols + 3) / 4 : 16)), dim3(kBlock), 0, st, first, V, (int)D, chunk, n_chunks, key,
+                         scale, partial, (T *)dtable);
     else
-      hipLaunchKernelGGL((embedding_join_kernel<T, 1>), dim3((unsigned)(n_chunks - 1), (unsigned)(cols < 16 ? cols : 16)), dim3(kBlock), 0, st, n, V, (int)D, chunk, n_chunks, key, scale,
-                         partial, (T *)dtable);
+      hipLaunchKernelGGL((embedding_join_kernel<T, 1>), dim3(borders, (unsigned)(cols < 16 ? cols : 16)), dim3(kBlock), 0, st, first, V, (int)D, chunk, n_chunks, key, scale, partial,
+                         (T *)dtable);
+    if (check_launch() != DGS_OK) return DGS_ELAUNCH;
   }
-  return check_launch();
+  return DGS_OK;
 }
 
 }  // namespace dgs

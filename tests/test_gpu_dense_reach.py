@@ -123,3 +123,21 @@ def test_matmul_fp8_of_every_sequence_s_last_token(L, K):
     assert a.stride(0) * 256 > 2 ** 31
     out = check_mm8(a, sa, b, sb, torch.bfloat16)
     assert torch.equal(out, dgsparse.matmul_fp8(a.view(torch.uint8).contiguous().view(a.dtype), sa.contiguous(), b, sb, torch.bfloat16))
+
+
+# ---- long lists -----------------------------------------------------------------------------------------------------------------
+def test_embedding_gradient_of_more_than_2_30_positions():
+    """A frequent token's partial sums are joined at the borders of chunks of 64: behind position 2^30 they are more than a launch has workgroups.
+    Token 999's places, sorted, run from 2^30 - 5 to the list's end.  Whole numbers: every sum is exact."""
+    import dgsparse
+    n, V = 2 ** 30 + 100, 1000
+    ids = torch.arange(n, dtype=torch.int32, device='cuda').remainder_(999)
+    ids[torch.arange(105, device='cuda') * 10000019] = 999
+    dout = torch.arange(n, dtype=torch.int32, device='cuda').remainder_(3).to(torch.float32).view(n, 1)
+    table = torch.zeros(V, 1, device='cuda', requires_grad=True)
+    grad, = torch.autograd.grad(dgsparse.embedding(ids, table, scale=0.5), table, dout)
+    want = torch.zeros(V, dtype=torch.float64, device='cuda')
+    for at in range(0, n, 1 << 27):
+        want += torch.bincount(ids[at:at + (1 << 27)], weights=dout[at:at + (1 << 27), 0].double(), minlength=V)
+    assert want.max() < 2 ** 24 and int((ids == 999).sum()) == 105
+    assert torch.equal(grad[:, 0].double(), 0.5 * want)
