@@ -490,7 +490,8 @@ extern "C" int dgs_embedding(int dtype, int id_bytes, int64_t n, int64_t V, int6
 }
 
 extern "C" size_t dgs_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D) {
-  if (n <= 0 || V < 0 || D <= 0) return 256;
+  if (embedding_sizes(DGS_F32, 4, n, V, D) != DGS_OK) return 0;  // (sizes that the entry refuses)
+  if (n == 0) return 256;
   return bwd_layout(n, V, D).total;
 }
 
