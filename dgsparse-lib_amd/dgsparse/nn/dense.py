@@ -66,6 +66,19 @@ class LinearFP8(torch.nn.Module):
         self.register_buffer('weight_scale', scale)
         self.out_dtype = out_dtype
 
+    def _apply(self, fn, recurse=True):
+        # half(), to(dtype) and their like change what is trained and multiplied in that type: the 8-bit values and their scales go along as the
+        # whole numbers of their bits, which a change of device moves and a change of type leaves alone
+        kept = {}
+        for name in ('weight', 'weight_scale'):
+            held = self._buffers[name]
+            bits = held.view({1: torch.uint8, 4: torch.int32}[held.element_size()])
+            moved = fn(bits)
+            kept[name] = (moved if moved.dtype == bits.dtype else bits.to(moved.device)).view(held.dtype)
+        super()._apply(fn, recurse)
+        self._buffers.update(kept)
+        return self
+
     def forward(self, x) -> torch.Tensor:
         q, scale = x if isinstance(x, tuple) else dense.quantize_fp8(x)
         return dense.matmul_fp8(q, scale, self.weight, self.weight_scale, self.out_dtype)
