@@ -66,6 +66,12 @@ class LinearFP8(torch.nn.Module):
         self.register_buffer('weight_scale', scale)
         self.out_dtype = out_dtype
 
+    def requantize(self, weight: torch.Tensor) -> None:
+        """The 8-bit values of another weight of the same shape, in place."""
+        q, scale = dense.quantize_fp8(weight.detach(), 128)
+        self.weight.view(torch.uint8).copy_(q.view(torch.uint8))
+        self.weight_scale.copy_(scale)
+
     def _apply(self, fn, recurse=True):
         # half(), to(dtype) and their like change what is trained and multiplied in that type: the 8-bit values and their scales go along as the
         # whole numbers of their bits, which a change of device moves and a change of type leaves alone
@@ -87,8 +93,9 @@ class LinearFP8(torch.nn.Module):
 class ResidualGCN(torch.nn.Module):
     """A residual graph layer with its norms in front: ``m = relu(A_hat (norm(x + r) W))``, ``out = ffn(norm(m + s))`` -> ``(out, s')`` where ``s``, ``s'``
     are the running residuals.  ``quantize()`` puts the graph projection into 8 bits for serving: the norm then writes 8-bit rows, which the
-    projection reads as they are.  The 8-bit weight is made once from the weight of that moment: training drops it, and after
-    ``load_state_dict`` it is to be made again."""
+    projection reads as they are.  The 8-bit weight is made from the weight, by ``quantize()`` and again behind
+    ``load_state_dict``; it is no part of a state dict, and training drops it.  A weight that is written to by other means in between is quantized again by
+    ``quantize()``."""
 
     def __init__(self, size: int, hidden_size: int, activation: str = 'silu', eps: float = 1e-6):
         super().__init__()
@@ -96,21 +103,45 @@ class ResidualGCN(torch.nn.Module):
         self.conv = GCNConv(size, size, activation='relu')
         self.ffn = GatedFFN(size, hidden_size, activation=activation)
         self.conv8 = None
+        self.in_8_bits = False
+        self.register_load_state_dict_post_hook(ResidualGCN._weight_loaded)
 
     def quantize(self) -> 'ResidualGCN':
-        self.conv8 = LinearFP8(self.conv.W.weight)
+        self.in_8_bits = True
+        if self.conv8 is None:
+            self.projection8()
+        else:
+            self.conv8.requantize(self.conv.W.weight)
         return self.eval()
+
+    def projection8(self) -> LinearFP8:
+        if self.conv8 is None:
+            self.conv8 = LinearFP8(self.conv.W.weight)
+            for name, held in list(self.conv8.named_buffers()):  # made of the weight: no part of a state dict
+                self.conv8.register_buffer(name, held, persistent=False)
+        return self.conv8
 
     def train(self, mode: bool = True) -> 'ResidualGCN':
         if mode:
-            self.conv8 = None
+            self.in_8_bits, self.conv8 = False, None
         return super().train(mode)
 
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        for key in [k for k in state_dict if k.startswith(prefix + 'conv8.')]:  # (written when they were a part of it)
+            del state_dict[key]
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
+
+    def _weight_loaded(self, _keys) -> None:
+        if self.conv8 is not None and self.conv.W.weight.is_cuda:
+            self.conv8.requantize(self.conv.W.weight)  # in place: a captured graph reads it where it is
+        else:
+            self.conv8 = None  # (made again where it is used)
+
     def forward(self, dcsr, x: torch.Tensor, residual: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-        if self.conv8 is not None:
+        if self.in_8_bits:
             with torch.no_grad():
                 q, scale, s = dense.add_rms_norm_fp8(x, residual, self.norm1.weight, self.norm1.eps)
-                m = spmm_sum_fused(dcsr, self.conv8((q, scale)), relu=True)
+                m = spmm_sum_fused(dcsr, self.projection8()((q, scale)), relu=True)
                 y, s = self.norm2(m, s)
                 return self.ffn(y), s
         y, s = self.norm1(x, residual)

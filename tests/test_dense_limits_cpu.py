@@ -45,3 +45,47 @@ def test_a_change_of_type_leaves_an_8_bit_weight_alone(quantize_here, change):
     assert lin.weight_scale.dtype == torch.float32 and torch.equal(lin.weight_scale, scale)
     assert list(lin.state_dict()) == ['weight', 'weight_scale']
     assert lin.to('meta').weight.is_meta and lin.weight.dtype == torch.float8_e4m3fn  # another device is one
+
+
+def test_a_loaded_weight_is_the_one_an_8_bit_projection_uses(quantize_here):
+    """load_state_dict in 8 bits: a plain checkpoint, one that was written in 8 bits, one of the time when the 8-bit values were a part of it, and one that lies
+    in a larger model's."""
+    import dgsparse.nn as nn
+
+    def projection(layer):
+        p = layer.projection8()
+        return p.weight.view(torch.uint8), p.weight_scale
+
+    torch.manual_seed(3)
+    plain, layer = nn.ResidualGCN(40, 16), nn.ResidualGCN(40, 16).quantize()
+    before = [v.clone() for v in projection(layer)]
+    q, scale = quantize_here(plain.conv.W.weight, 128)
+    assert not torch.equal(before[0], q.view(torch.uint8))
+    written = nn.ResidualGCN(40, 16)
+    written.load_state_dict(plain.state_dict())
+    assert list(written.quantize().state_dict()) == list(plain.state_dict())
+    older = {**plain.state_dict(), 'conv8.weight': torch.zeros(40, 40).to(torch.float8_e4m3fn), 'conv8.weight_scale': torch.ones(1, 1)}
+    for state in (plain.state_dict(), written.state_dict(), older):
+        layer = nn.ResidualGCN(40, 16).quantize()
+        layer.load_state_dict(state)
+        assert torch.equal(projection(layer)[0], q.view(torch.uint8)) and torch.equal(projection(layer)[1], scale)
+        assert torch.equal(layer.conv.W.weight, plain.conv.W.weight)
+        fresh = nn.ResidualGCN(40, 16)  # in full precision it stays so
+        fresh.load_state_dict(state)
+        assert fresh.conv8 is None and not fresh.in_8_bits
+    model = torch.nn.Sequential(torch.nn.Linear(2, 2), layer)
+    model.load_state_dict({**model.state_dict(), '1.conv.W.weight': 2 * plain.conv.W.weight.detach()})
+    assert torch.equal(projection(layer)[1], 2 * scale)
+    layer.load_state_dict({}, strict=False)
+    assert torch.equal(projection(layer)[1], 2 * scale)
+    with pytest.raises(RuntimeError, match='Missing key'):
+        layer.load_state_dict({})
+    import copy
+    twin = copy.deepcopy(layer)
+    twin.load_state_dict(plain.state_dict())
+    assert torch.equal(projection(twin)[1], scale) and torch.equal(projection(layer)[1], 2 * scale)
+    with torch.no_grad():
+        layer.conv.W.weight.copy_(plain.conv.W.weight)
+    assert torch.equal(projection(layer.quantize())[1], scale)
+    layer.train()
+    assert layer.conv8 is None and not layer.in_8_bits
