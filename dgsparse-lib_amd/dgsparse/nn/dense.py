@@ -15,6 +15,8 @@ class Embedding(torch.nn.Module):
 
     def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None, scale: float = 1.0):
         super().__init__()
+        if padding_idx is not None and not 0 <= padding_idx < num_embeddings:
+            raise ValueError(f'dgsparse: padding_idx {padding_idx} is not a row of the table')
         self.padding_idx, self.scale = padding_idx, scale
         self.weight = torch.nn.Parameter(torch.randn(num_embeddings, embedding_dim))
         if padding_idx is not None:

@@ -89,3 +89,11 @@ def test_a_loaded_weight_is_the_one_an_8_bit_projection_uses(quantize_here):
     assert torch.equal(projection(layer.quantize())[1], scale)
     layer.train()
     assert layer.conv8 is None and not layer.in_8_bits
+
+
+def test_embedding_layer_refuses_a_padding_row_that_no_call_takes():
+    import dgsparse.nn as nn
+    for bad in (-1, 10):
+        with pytest.raises(ValueError, match='padding_idx'):
+            nn.Embedding(10, 4, padding_idx=bad)
+    assert nn.Embedding(10, 4, padding_idx=9).weight[9].eq(0).all() and nn.Embedding(10, 4).padding_idx is None
