@@ -414,6 +414,15 @@ extern "C" size_t dgs_matmul_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K
   return a > b ? a : b;
 }
 
+extern "C" int dgs_matmul_fp8_tiles(int out_dtype, int64_t M, int64_t N, int64_t K, int32_t *out) {
+  if (!dtype_ok(out_dtype) || M < 0 || N < 0 || K <= 0 || !out) return DGS_EINVAL;
+  if (!sizes8_ok(M, N, K)) return DGS_ERANGE;
+  const TilePlan p = layout8(M, N, K, out_dtype != DGS_F32).plan;
+  out[0] = few_rows(M, N, K) ? 0 : p.shape == kBig ? 256 : p.shape == kMid ? 128 : 64;
+  out[1] = p.splits;
+  return DGS_OK;
+}
+
 extern "C" int dgs_matmul_fp8(int out_dtype, int64_t M, int64_t N, int64_t K, const uint8_t *a, int64_t lda, const float *a_scale, const uint8_t *b, int64_t ldb,
                               const float *b_scale, void *out, void *workspace, size_t workspace_bytes, dgsStream_t stream) {
   if (!dtype_ok(out_dtype) || M < 0 || N < 0 || K <= 0 || lda < 0 || ldb < 0) return DGS_EINVAL;

@@ -278,6 +278,21 @@ static bool fits(int64_t M, int64_t N) {  // tiles of the smallest shape in a la
   return ((M + 63) / 64) * ((N + 31) / 32) < INT32_MAX;
 }
 
+// The products' tiles.  Forward (backward, made again: cols = the padded F): no split, the activation needs whole sums; 32 bits: no largest tile (three
+// planes of 256 + 256 rows leave no room for a second workgroup).
+template <typename T>
+static TilePlan plan_gated(int64_t rows, int64_t cols, int64_t D) {
+  return tile_plan(rows, cols, (D + kStepK<T> - 1) / kStepK<T>, 1, true, sizeof(T) == 2, false);
+}
+template <typename T>
+static TilePlan plan_dx(int64_t rows, int64_t D, int64_t F) {
+  return tile_plan(rows, D, 2 * ((F + kStepK<T> - 1) / kStepK<T>), 1, false, sizeof(T) == 2, true);
+}
+template <typename T>
+static TilePlan plan_dw(int64_t rows, int64_t D, int64_t F) {
+  return tile_plan(F, D, (rows + kStepK<T> - 1) / kStepK<T>, 2, false, sizeof(T) == 2, true);
+}
+
 struct Layout {
   bool pad;          // x and the weights are copied into padded rows
   int64_t ldx, ldg;  // in elements: of x and the weights, and of dg and du
@@ -299,9 +314,7 @@ static Layout layout(int64_t rows, int64_t D, int64_t F, bool backward, int64_t 
   L.du = take(backward ? (size_t)rows * L.ldg * sizeof(T) : 0);
   size_t part = 0;
   if (backward) {
-    constexpr int kK = kStepBytes / (int)sizeof(T);
-    const TilePlan px = tile_plan(rows, D, 2 * ((F + kK - 1) / kK), 1, false, sizeof(T) == 2, true);
-    const TilePlan pw = tile_plan(F, D, (rows + kK - 1) / kK, 2, false, sizeof(T) == 2, true);
+    const TilePlan px = plan_dx<T>(rows, D, F), pw = plan_dw<T>(rows, D, F);
     const size_t bx = px.splits > 1 ? (size_t)px.splits * rows * D * 4 : 0, bw = pw.splits > 1 ? (size_t)pw.splits * 2 * F * D * 4 : 0;
     part = bx > bw ? bx : bw;
   }
@@ -330,10 +343,8 @@ static int operands(int64_t rows, int64_t D, int64_t F, const void *x, int64_t l
 
 template <typename T, int ACT, bool BWD>
 static int launch_gated(int64_t rows, int64_t D, int64_t F, const Operands<T> &op, const GatedOut &out, hipStream_t st) {
-  constexpr int kK = kStepBytes / (int)sizeof(T);
-  const int64_t cols = BWD ? out.ldo : F;
-  constexpr bool kWide = sizeof(T) == 2;  // (32 bits: three planes of 256 + 256 rows leave no room for a second workgroup)
-  const TilePlan p = tile_plan(rows, cols, (D + kK - 1) / kK, 1, true, kWide, false);
+  constexpr bool kWide = sizeof(T) == 2;
+  const TilePlan p = plan_gated<T>(rows, BWD ? out.ldo : F, D);
   GemmArgs g = {{op.x, nullptr}, {op.wg, op.wu}, op.ldx * (int64_t)sizeof(T), op.ldw * (int64_t)sizeof(T), rows, F, D, p.tiles_m, p.tiles_n, 1};
   if (!grid_ok((int64_t)p.tiles_m * p.tiles_n, p.shape == kBig ? 512 : 256)) return DGS_ERANGE;
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n));
@@ -416,7 +427,6 @@ static int ffn_bwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ld
   int rc = operands<T>(rows, D, F, x, ldx, wg, wu, ldw, ws, L, st, op);
   if (rc != DGS_OK) return rc;
   constexpr int64_t size = sizeof(T);
-  constexpr int kK = kStepBytes / (int)sizeof(T);
   char *dg = ws + L.dg, *du = ws + L.du;
   const GatedOut out = {dh, const_cast<float *>(pre), dg, du, F, L.ldg};
   if (pre) {
@@ -437,14 +447,25 @@ static int ffn_bwd(int64_t rows, int64_t D, int64_t F, const void *x, int64_t ld
   if (rc == DGS_OK && dx) {  // dx [rows, D] = dg Wg + du Wu: K = F, the weights K-outer
     GemmArgs g = {{dg, du}, {op.wg, op.wu}, L.ldg * size, op.ldw * size, rows, D, F, 0, 0, 1};
     PlainOut o = {{dx, nullptr}, D, nullptr};
-    rc = launch_product<T, false, true, kSum>(g, o, tile_plan(rows, D, 2 * ((F + kK - 1) / kK), 1, false, size == 2, true), partial, st);
+    rc = launch_product<T, false, true, kSum>(g, o, plan_dx<T>(rows, D, F), partial, st);
   }
   if (rc == DGS_OK && dwg) {  // dWg, dWu [F, D] = dg^T x, du^T x: K = rows, both operands K-outer
     GemmArgs g = {{dg, du}, {op.x, nullptr}, L.ldg * size, op.ldx * size, F, D, rows, 0, 0, 1};
     PlainOut o = {{dwg, dwu}, D, nullptr};
-    rc = launch_product<T, true, true, kTwo>(g, o, tile_plan(F, D, (rows + kK - 1) / kK, 2, false, size == 2, true), partial, st);
+    rc = launch_product<T, true, true, kTwo>(g, o, plan_dw<T>(rows, D, F), partial, st);
   }
   return rc;
+}
+
+static int edge(Shape s) { return s == kBig ? 256 : s == kMid ? 128 : 64; }
+template <typename T>
+static void tiles(int64_t rows, int64_t D, int64_t F, int32_t *out) {
+  const TilePlan p[] = {plan_gated<T>(rows, F, D), plan_dx<T>(rows, D, F), plan_dw<T>(rows, D, F)};
+  for (int i = 0; i < 3; i++) {
+    out[2 * i] = edge(p[i].shape);
+    out[2 * i + 1] = p[i].splits;
+  }
+  if (few_rows<T>(rows, F)) out[0] = 0;
 }
 
 }  // namespace dgs
@@ -463,6 +484,15 @@ static int ffn_sizes(int dtype, int activation, int64_t rows, int64_t D, int64_t
 extern "C" size_t dgs_gated_ffn_workspace_bytes(int dtype, int64_t rows, int64_t D, int64_t F, int backward) {
   if (!dtype_ok(dtype) || rows <= 0 || D <= 0 || F <= 0) return 0;
   return dtype == DGS_F32 ? layout<float>(rows, D, F, backward, D).total : layout<f16>(rows, D, F, backward, D).total;
+}
+
+extern "C" int dgs_gated_ffn_tiles(int dtype, int64_t rows, int64_t D, int64_t F, int32_t *out) {
+  const int rc = ffn_sizes(dtype, DGS_ACT_SILU, rows, D, F, 0, 0);
+  if (rc != DGS_OK) return rc;
+  if (!out) return DGS_EINVAL;
+  if (dtype == DGS_F32) tiles<float>(rows, D, F, out);
+  else tiles<f16>(rows, D, F, out);
+  return DGS_OK;
 }
 
 #define DGS_ACTS(T, CALL)                                      \

@@ -157,7 +157,7 @@ EXPORTS = ['dgs_version', 'dgs_arch', 'dgs_strerror', 'dgs_reload_tuning', 'dgs_
            # dense operators: bound by csrc/torch_dense.cpp (dgsparse/dense.py), not through ctypes
            'dgs_embedding', 'dgs_embedding_bwd_workspace_bytes', 'dgs_embedding_bwd', 'dgs_rms_norm', 'dgs_rms_norm_bwd_workspace_bytes',
            'dgs_rms_norm_bwd', 'dgs_gated_ffn_workspace_bytes', 'dgs_gated_ffn', 'dgs_gated_ffn_bwd', 'dgs_quantize_fp8',
-           'dgs_matmul_fp8_workspace_bytes', 'dgs_matmul_fp8']
+           'dgs_matmul_fp8_workspace_bytes', 'dgs_matmul_fp8', 'dgs_gated_ffn_tiles', 'dgs_matmul_fp8_tiles']
 
 
 # ---- DGS_CANARY=1 (debug): every output and workspace this module allocates sits between two 4 KiB guard bands of a

@@ -473,6 +473,10 @@ int dgs_gated_ffn_bwd(int dtype, int activation, int64_t rows, int64_t D, int64_
                       const void *w_up, int64_t ldw, const float *pre, const void *dh, void *dx, void *dw_gate, void *dw_up, void *workspace,
                       size_t workspace_bytes, dgsStream_t stream);
 
+/* Which tiles these sizes take on the current device, for tests and timing (as dgs_spmm_csr_schedule): out[2 i] the tile's edge - 256, 128, 64, or 0 for
+ * the kernel of few rows - and out[2 i + 1] the splits of K, of the forward product, dx and dWg / dWu. */
+int dgs_gated_ffn_tiles(int dtype, int64_t rows, int64_t D, int64_t F, int32_t *out);
+
 /* x [rows, cols] in 8-bit floating point (e4m3): q [rows, cols] contiguous, scales [ceil(rows / block_rows), ceil(cols / 128)], one for each
  * block_rows (1 or 128) x 128 values: max|x| / 448 (at least 2^-96 / 448; NaN if one of the values is), q = x / scale. */
 int dgs_quantize_fp8(int dtype, int64_t rows, int64_t cols, const void *x, int64_t ldx, int block_rows, uint8_t *q, float *scales,
@@ -483,6 +487,8 @@ int dgs_quantize_fp8(int dtype, int64_t rows, int64_t cols, const void *x, int64
 size_t dgs_matmul_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int dgs_matmul_fp8(int out_dtype, int64_t M, int64_t N, int64_t K, const uint8_t *a, int64_t lda, const float *a_scale, const uint8_t *b,
                    int64_t ldb, const float *b_scale, void *out, void *workspace, size_t workspace_bytes, dgsStream_t stream);
+/* The tile's edge (0: the kernel of few rows) and the splits of K that these sizes take on the current device. */
+int dgs_matmul_fp8_tiles(int out_dtype, int64_t M, int64_t N, int64_t K, int32_t *out);
 
 /* ---- GE-SpMM / SDDMM compatibility entry points (same names and argument order as the reference's
  *      standalone C libraries; default stream, void return) ------------------------------------- */

@@ -97,3 +97,14 @@ def test_embedding_layer_refuses_a_padding_row_that_no_call_takes():
         with pytest.raises(ValueError, match='padding_idx'):
             nn.Embedding(10, 4, padding_idx=bad)
     assert nn.Embedding(10, 4, padding_idx=9).weight[9].eq(0).all() and nn.Embedding(10, 4).padding_idx is None
+
+
+def test_tiles_entries_refuse_what_the_products_refuse():
+    import ctypes
+    lib = ctypes.CDLL(os.path.join(ROOT, 'dgsparse-lib_amd', 'dgsparse', 'libdgsparse_hip.so'))
+    out = (ctypes.c_int32 * 6)()
+    for f in (lib.dgs_gated_ffn_tiles, lib.dgs_matmul_fp8_tiles):
+        f.argtypes = [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_void_p]
+        assert f(0, 5, 64, 64, ctypes.addressof(out)) == 0 and out[0] == 0
+        assert f(9, 5, 64, 64, ctypes.addressof(out)) == -1 and f(0, -1, 64, 64, ctypes.addressof(out)) == -1 and f(0, 5, 64, 64, None) == -1
+        assert f(0, 2 ** 40, 64, 64, ctypes.addressof(out)) == -4
