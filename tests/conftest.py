@@ -28,17 +28,17 @@ def _has_gpu():
         return False
 
 
-# Tests that hold a wrong value, kept as they are: name -> the proof.
+# Tests that hold a wrong value, kept as they are: name -> the proof (and the test that holds the right one).
 HOLDS_A_WRONG_VALUE = {
     'test_storage_tells_the_launches_its_longest_row_and_column': 'sets DGS_HUB_CHAIN=200 and takes a row of 280 for a hub row; the threshold is clamped to '
-                                                                 '1024 and above (include/dgsparse_hip.h), so the row is none and keeps its hint',
+                                                                 '1024 and above (include/dgsparse_hip.h), so the row is none and keeps its hint (test_gpu_hub_hints.py: the same with 1300 and 1024)',
 }
 
 
 def pytest_collection_modifyitems(config, items):
     for item in items:
         if item.name in HOLDS_A_WRONG_VALUE:
-            item.add_marker(pytest.mark.xfail(reason=HOLDS_A_WRONG_VALUE[item.name], strict=False))
+            item.add_marker(pytest.mark.xfail(reason=HOLDS_A_WRONG_VALUE[item.name], strict=True))
     # stable: everything else keeps its file / definition order, the first-contact tests move behind it (the driver runs
     # `pytest -x`: the library's default is protected by the device self-test, the tests that FORCE the gated schedules are not)
     items.sort(key=lambda it: 1 if 'first_contact' in it.keywords else 0)
