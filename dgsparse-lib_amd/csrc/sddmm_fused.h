@@ -53,6 +53,13 @@ __device__ __forceinline__ float tb8(const float (&pt)[8], int lig) {
   return tot;
 }
 
+// What steers a wave is the same in all its lanes, and is kept where the compiler knows that it is: in scalar registers, so that every loop below
+// ends by a scalar branch.  As vector values (a shuffle's result, the wave's number from threadIdx) they made each loop a divergent one, whose
+// way out has an empty exec mask until the mask of the loop's entry is put back; hipcc 7.2, built without packed fp32 instructions, spilled the wave's row
+// count and reloaded it in front of that: the reload loaded nothing, the register held gathered features, and the loop over the rows did not end
+// (66 000 x 1000, 256 features).  tests/test_isa_exec_cpu.py looks for such reloads in every kernel of the library.
+__device__ __forceinline__ int wave_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 struct SfLds {
   int2 tile[kBlock / kWave][kCap];   // {col, local row} of a staged run (row blocks) / {col, -} of a unit's 64-nnz tile
   float res[kBlock / kWave][kCap];   // results of the run, stored coalesced at its end
@@ -67,19 +74,19 @@ __device__ __forceinline__ void sddmm_units_body(int bid, int nblocks, SfLds &ld
                                                  const float *__restrict__ D2, const int *__restrict__ E,
                                                  float *__restrict__ out, const UnitTab &ut) {
   constexpr int NG = kWave / G;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = wave_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane / G, l = lane % G;
   int2 *tile = lds.tile[wave];
   float *res = lds.res[wave];
   const int f0 = l * V;
   const bool fl = f0 < F;
   const int fo = fl ? f0 : 0;
-  const int n_units = *ut.n_units;
+  const int n_units = wave_uniform(*ut.n_units);
   int u, uend, wstride;
   if ((nblocks & 7) == 0) {  // XCD x walks slice x of the (sorted) unit table: block b runs on XCD b % 8 (speed hint)
     const int x = bid & 7;
-    const int lo = ut.xcd_start ? ut.xcd_start[x] : (int)(((long long)n_units * x) >> 3);
-    uend = ut.xcd_start ? ut.xcd_start[x + 1] : (int)(((long long)n_units * (x + 1)) >> 3);
+    const int lo = ut.xcd_start ? wave_uniform(ut.xcd_start[x]) : (int)(((long long)n_units * x) >> 3);
+    uend = ut.xcd_start ? wave_uniform(ut.xcd_start[x + 1]) : (int)(((long long)n_units * (x + 1)) >> 3);
     u = lo + (bid >> 3) * (kBlock / kWave) + wave;
     wstride = (nblocks >> 3) * (kBlock / kWave);
   } else {
@@ -89,19 +96,20 @@ __device__ __forceinline__ void sddmm_units_body(int bid, int nblocks, SfLds &ld
   }
   const int ent = tb8_entry(l);
   for (; u < uend; u += wstride) {
-    const int4 d = ut.units[u];  // {row, first nnz, nnz in the unit, -}
+    const int4 du = ut.units[u];  // {row, first nnz, nnz in the unit, -}
+    const int row = wave_uniform(du.x), first = wave_uniform(du.y), end = first + wave_uniform(du.z);
     float a[V];
     int m[V];
-    load_vec_rowop<V>(D1 + (int64_t)d.x * F + fo, a);
-    if constexpr (MASK) load_vec<V>(E + (int64_t)d.x * F + fo, m);
+    load_vec_rowop<V>(D1 + (int64_t)row * F + fo, a);
+    if constexpr (MASK) load_vec<V>(E + (int64_t)row * F + fo, m);
     float scale = 1.0f;
-    if constexpr (MEAN) scale = (float)(rowptr[d.x + 1] - rowptr[d.x]);
+    if constexpr (MEAN) scale = (float)(rowptr[row + 1] - rowptr[row]);
     if (!fl) {
 #pragma unroll
       for (int v = 0; v < V; v++) a[v] = 0.0f;
     }
-    for (int t0 = d.y; t0 < d.y + d.z; t0 += kWave) {
-      const int cnt = min(kWave, d.y + d.z - t0);
+    for (int t0 = first; t0 < end; t0 += kWave) {
+      const int cnt = min(kWave, end - t0);
       __builtin_amdgcn_wave_barrier();
       if (lane < cnt) tile[lane].x = ld_stream(col + t0 + lane);
       __builtin_amdgcn_wave_barrier();
@@ -143,7 +151,7 @@ __device__ __forceinline__ void sddmm_rows_body(int bid, int rpw, SfLds &lds, in
                                                 const float *__restrict__ D2, const int *__restrict__ E,
                                                 float *__restrict__ out) {
   constexpr int NG = kWave / G;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = wave_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane / G, l = lane % G;
   const int r0 = (bid * (kBlock / kWave) + wave) * rpw;
   if (r0 >= M) return;  // wave-uniform
@@ -168,7 +176,7 @@ __device__ __forceinline__ void sddmm_rows_body(int bid, int rpw, SfLds &lds, in
 
   int a = 0;
   while (a < nrows) {
-    const int s_a = __shfl(s_i, a, 64);
+    const int s_a = wave_uniform(__shfl(s_i, a, 64));
     // first row >= a that cannot join the run: long, or it would overflow the LDS tile, or past the end
     const unsigned long long brk = __ballot(lane >= a && (long_i || (e_i - s_a) > kCap || lane >= nrows));
     const int b = brk ? (__ffsll((long long)brk) - 1) : kRowsPerWave;
@@ -176,7 +184,7 @@ __device__ __forceinline__ void sddmm_rows_body(int bid, int rpw, SfLds &lds, in
       a++;
       continue;
     }
-    const int e_b = __shfl(e_i, b - 1, 64);
+    const int e_b = wave_uniform(__shfl(e_i, b - 1, 64));
     const int cnt = e_b - s_a;
     if (cnt == 0) {
       a = b;
@@ -205,13 +213,15 @@ __device__ __forceinline__ void sddmm_rows_body(int bid, int rpw, SfLds &lds, in
     }
     __builtin_amdgcn_wave_barrier();
     // ---- group g takes the contiguous range [ps, pe) of the run, 8 nnz per batch
-    const int ps = (int)(((long long)g * cnt) / NG), pe = (int)(((long long)(g + 1) * cnt) / NG);
-    for (int p = ps; p < pe; p += kSfU) {
+    //      (every group makes the wave's number of batches: beyond its own range it repeats its last nnz and stores nothing)
+    const int ps = (int)(((long long)g * cnt) / NG), pe = (int)(((long long)(g + 1) * cnt) / NG), at = max(pe - 1, 0);
+    for (int p0 = 0; p0 < (cnt + NG - 1) / NG; p0 += kSfU) {
+      const int p = ps + p0;
       int2 cr[kSfU];
       float av[kSfU][V], b[kSfU][V], pt[kSfU];
       int mv[kSfU][V];
 #pragma unroll
-      for (int q = 0; q < kSfU; q++) cr[q] = tile[min(p + q, pe - 1)];
+      for (int q = 0; q < kSfU; q++) cr[q] = tile[min(p + q, at)];
 #pragma unroll
       for (int q = 0; q < kSfU; q++) load_vec_gather<V>(D2 + (int64_t)cr[q].x * F + fo, b[q]);
       // D1 slices: consecutive nnz share their row, so most of these are the same address and hit L1 (rows are consecutive:
@@ -247,7 +257,8 @@ __device__ __forceinline__ void sddmm_rows_body(int bid, int rpw, SfLds &lds, in
       if (l < 8 && p + ent < pe) res[p + ent] = tot;
     }
     __builtin_amdgcn_wave_barrier();
-    for (int t = lane; t < cnt; t += kWave) out[s_a + t] = res[t];
+    for (int t0 = 0; t0 < cnt; t0 += kWave)
+      if (t0 + lane < cnt) out[s_a + t0 + lane] = res[t0 + lane];
     __builtin_amdgcn_wave_barrier();
     a = b;
   }
