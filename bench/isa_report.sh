@@ -9,7 +9,7 @@ set -e
 cd "$(dirname "$0")/../dgsparse-lib_amd/csrc"
 T=$(mktemp -d)
 for tu in v4a v4b; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -I../../include --cuda-device-only -c spmm_$tu.hip -o $T/$tu.co 2>/dev/null &
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -I../../include -Xclang -target-feature -Xclang -packed-fp32-ops --cuda-device-only -c spmm_$tu.hip -o $T/$tu.co 2>/dev/null &
 done
 wait
 : > $T/notes

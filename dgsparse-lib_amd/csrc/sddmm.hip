@@ -78,6 +78,9 @@ __device__ __forceinline__ void sd_tile_dots(const int2 *tile, int *cnt, int cnt
           load_vec<V>(D2 + (int64_t)cr[q].x * F + f, b[q]);
           if constexpr (MASK && !ONE_ROW) load_vec<V>(E + (int64_t)cr[q].y * F + f, m[q]);
         }
+        // every load is on its way before the first product: among them the scheduler puts products between the loads, which then wait for each other
+        // (products-shaped graph, 64 features: 2674 us for 2236)
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < kSdU; q++)
 #pragma unroll

@@ -1290,7 +1290,10 @@ __device__ __forceinline__ void spmm_units_body(int bid, int nblocks, RowsLds &l
 #ifndef DGS_WAVES_ARG
 #define DGS_WAVES_ARG 5
 #endif
-constexpr int fused_waves_per_simd(int op) { return (op == DGS_MAX || op == DGS_MIN) ? DGS_WAVES_ARG : DGS_WAVES_SUM; }
+// (The opt-in fold twins of min and mean hold the ticket state as well: one wave less, instead of 12 - 42 spilled registers.)
+constexpr int fused_waves_per_simd(int op, bool fold) {
+  return ((op == DGS_MAX || op == DGS_MIN) ? DGS_WAVES_ARG : DGS_WAVES_SUM) - (fold && (op == DGS_MIN || op == DGS_MEAN) ? 1 : 0);
+}
 
 // Fused launch: blocks [0, nbu) walk the unit table of the huge rows (persistent, strided), the remaining blocks
 // each own 4 x 64 consecutive rows.  Unit blocks come first so that the longest-running work starts first; the
@@ -1316,7 +1319,7 @@ struct FusedLds<true> {
   __device__ FusedLds() {}
 };
 template <int G, int V, int OP, bool HAS_VAL, bool ACC = false, bool HUB = false, bool FOLD = false>
-__global__ __launch_bounds__(kBlock, fused_waves_per_simd(OP)) void spmm_fused(int M, int N, int nbh, int nbu, int rpw, const int *__restrict__ rowptr,
+__global__ __launch_bounds__(kBlock, fused_waves_per_simd(OP, FOLD)) void spmm_fused(int M, int N, int nbh, int nbu, int rpw, const int *__restrict__ rowptr,
                                                      const int *__restrict__ col, const float *__restrict__ val,
                                                      const float *__restrict__ B, float *__restrict__ C,
                                                      int *__restrict__ E, const UnitTab ut, float *__restrict__ part,
