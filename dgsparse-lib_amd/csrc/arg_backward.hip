@@ -174,8 +174,8 @@ extern "C" int dgs_spmm_arg_backward_f32(int64_t M, int64_t K, int64_t N, int64_
   if (M < 0 || K < 0 || N < 0 || nnz < 0) return DGS_EINVAL;
   if (M >= INT32_MAX || K >= INT32_MAX || N >= INT32_MAX || nnz >= INT32_MAX) return DGS_ERANGE;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (gX && K > 0 && N > 0 && hipMemsetAsync(gX, 0, (size_t)K * N * sizeof(float), st) != hipSuccess) return DGS_ELAUNCH;
-  if (gW && nnz > 0 && hipMemsetAsync(gW, 0, (size_t)nnz * sizeof(float), st) != hipSuccess) return DGS_ELAUNCH;
+  if (gX && K > 0 && N > 0 && fill_words(gX, 0u, (size_t)K * N * sizeof(float), st) != DGS_OK) return DGS_ELAUNCH;
+  if (gW && nnz > 0 && fill_words(gW, 0u, (size_t)nnz * sizeof(float), st) != DGS_OK) return DGS_ELAUNCH;
   if (M == 0 || N == 0 || nnz == 0 || (!gX && !gW)) return DGS_OK;
   if (!rowptr || !col || !E || !gC || (gW && !X)) return DGS_EINVAL;
   const bool al = is_aligned16(E) && is_aligned16(gC);

@@ -90,7 +90,7 @@ extern "C" int dgs_csr2csc_i32(int64_t M, int64_t Kcols, int64_t nnz, const int3
   if (cscval && !val) return DGS_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (nnz == 0) {
-    return hipMemsetAsync(colptr, 0, (size_t)(Kcols + 1) * 4, st) == hipSuccess ? DGS_OK : DGS_ELAUNCH;
+    return fill_words(colptr, 0u, (size_t)(Kcols + 1) * 4, st);
   }
   if (!rowptr || !col || !workspace) return DGS_EINVAL;
   const Csr2cscLayout L = layout(Kcols, nnz);

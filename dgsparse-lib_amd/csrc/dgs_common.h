@@ -304,6 +304,10 @@ inline bool is_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p)
 
 inline int check_launch() { return hipGetLastError() == hipSuccess ? DGS_OK : DGS_ELAUNCH; }
 
+// `bytes` (a multiple of 4) at p set to `word`, by a kernel (misc.hip): every entry may be recorded into a graph, and a graph's memset nodes have
+// given wrong results on this hardware from the second replay on.
+int fill_words(void *p, uint32_t word, size_t bytes, hipStream_t st);
+
 // Tuning overrides (tests and experiments; every one has a compiled-in default at its point of use).  The environment is read
 // ONCE per process into an immutable snapshot (misc.hip: std::call_once), so a launch costs no getenv() and host threads can
 // launch concurrently; dgs_reload_tuning() publishes a fresh snapshot (tests that flip DGS_PANEL* between calls).

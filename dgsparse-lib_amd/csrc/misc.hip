@@ -10,6 +10,21 @@
 
 namespace dgs {
 
+// ---- clearing (dgs_common.h) --------------------------------------------------------------------------------------------------
+static __global__ __launch_bounds__(kBlock) void fill_words_kernel(uint32_t *__restrict__ p, uint32_t word, int64_t words, int64_t pieces) {
+  const int64_t n = (int64_t)gridDim.x * kBlock, t = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int4 w = make_int4((int)word, (int)word, (int)word, (int)word);
+  for (int64_t i = t; i < pieces; i += n) reinterpret_cast<int4 *>(p)[i] = w;
+  for (int64_t i = 4 * pieces + t; i < words; i += n) p[i] = word;
+}
+int fill_words(void *p, uint32_t word, size_t bytes, hipStream_t st) {
+  if (bytes == 0) return DGS_OK;
+  const int64_t words = (int64_t)(bytes / 4), pieces = is_aligned16(p) ? words / 4 : 0, work = pieces ? pieces : words;
+  const int64_t blocks = (work + kBlock - 1) / kBlock;
+  hipLaunchKernelGGL(fill_words_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(kBlock), 0, st, static_cast<uint32_t *>(p), word, words, pieces);
+  return check_launch();
+}
+
 // ---- process-wide tuning snapshot + per-device facts (the only global state of the library; see dgs_common.h) -------------
 // Every publish is a fresh heap snapshot that is never written again and never freed (64 bytes per dgs_reload_tuning(), a
 // tests-only call): a launch that holds `const Tuning &` keeps valid, unchanging values however many reloads follow (

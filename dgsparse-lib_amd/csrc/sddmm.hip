@@ -387,7 +387,7 @@ static int launch_sddmm_panel(const SdPanelPlan &P, int64_t M, int64_t F, const 
   for (int64_t fb = 0; fb < F; fb += 256) {  // one sweep per 256-feature tile; later tiles add to out[]
     const int W = (int)(F - fb < 256 ? F - fb : 256);
     const int pass = (fb ? 1 : 0) | (fb + 256 >= F ? 2 : 0);
-    if (hipMemsetAsync(arrivals, 0, sizeof(int), st) != hipSuccess) return DGS_ELAUNCH;
+    if (fill_words(arrivals, 0u, sizeof(int), st) != DGS_OK) return DGS_ELAUNCH;
     hipLaunchKernelGGL(kern, dim3((unsigned)P.nwg), dim3(kPanelBlock), P.lds, st, (int)M, W, (int)F, pass, P.R, P.tlong,
                        P.pcols, P.npanels, P.nsb, P.lead, rowptr, col, D1 + fb, D2 + fb, E ? E + fb : nullptr, out,
                        arrivals);
@@ -417,7 +417,7 @@ static int run_sddmm(int64_t M, int64_t K, int64_t F, int64_t nnz, const int *ro
   if (M >= INT32_MAX || K >= INT32_MAX || F >= INT32_MAX || nnz >= INT32_MAX) return DGS_ERANGE;
   if (M == 0 || nnz == 0) return DGS_OK;
   if (!rowptr || !col || !out || (F > 0 && (!D1 || !D2)) || (MASK && !E)) return DGS_EINVAL;
-  if (F == 0) return hipMemsetAsync(out, 0, (size_t)nnz * sizeof(float), st) == hipSuccess ? DGS_OK : DGS_ELAUNCH;
+  if (F == 0) return fill_words(out, 0u, (size_t)nnz * sizeof(float), st);
   const bool al = is_aligned16(D1) && is_aligned16(D2) && (!MASK || is_aligned16(E));
   const FeatMap fm = feat_map(F, al);
   const SdPanelPlan P = sd_panel_plan(M, K, F, nnz, fm.tiles, fm.G, fm.V, MASK);
@@ -494,7 +494,7 @@ extern "C" int dgs_sddmm_coo_f32(int64_t F, int64_t nnz, const int32_t *rowind, 
   if (nnz == 0) return DGS_OK;
   if (!rowind || !colind || !out || (F > 0 && (!D1 || !D2))) return DGS_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (F == 0) return hipMemsetAsync(out, 0, (size_t)nnz * sizeof(float), st) == hipSuccess ? DGS_OK : DGS_ELAUNCH;
+  if (F == 0) return fill_words(out, 0u, (size_t)nnz * sizeof(float), st);
   const FeatMap fm = feat_map(F, is_aligned16(D1) && is_aligned16(D2));
   if (fm.V == 4) return dispatch_coo<4>(fm.G, F, fm.tiles, nnz, rowind, colind, D1, D2, out, st);
   return dispatch_coo<1>(fm.G, F, fm.tiles, nnz, rowind, colind, D1, D2, out, st);

@@ -93,7 +93,7 @@ constexpr int kU1 = DGS_KU1;   // rolling window of B-row gathers per lane in th
 #endif
 constexpr int kU = DGS_KU;     // gathers in flight per lane in the wave-cooperative unit loop
 
-struct SpmmWs {       // workspace header (zeroed every call with one 16-byte memset)
+struct SpmmWs {       // workspace header (zeroed every call)
   int n_units;        // K0 -> fused/K2: number of unit descriptors
   int n_pslots;       // partial-row slots handed out (multi-unit rows only)
   int arrivals;       // spmm_panel: panel steps finished, summed over workgroups (soft barrier)
@@ -1650,7 +1650,7 @@ static int launch_impl(const SpmmArgs &a) {
       float *part = reinterpret_cast<float *>(w + L.off_part);
       int *parte = reinterpret_cast<int *>(w + L.off_parte);
       UnitTab ut{&hdr->n_units, &hdr->n_long, nullptr, units, longrows};
-      if (hipMemsetAsync(hdr, 0, sizeof(SpmmWs), a.st) != hipSuccess) return DGS_ELAUNCH;
+      if (fill_words(hdr, 0u, sizeof(SpmmWs), a.st) != DGS_OK) return DGS_ELAUNCH;
       const int64_t k0b = (a.M + (int64_t)kBlock * kK0Rows - 1) / ((int64_t)kBlock * kK0Rows);
       int tl = P.tlong > L.ch ? P.tlong : L.ch;  // every long row has >= 2 units => all go through combine
       if (tl > 65534) tl = 65534;  // max keeps 16-bit arg positions (unit lengths never exceed 32768: still >= 2 units)
@@ -1679,7 +1679,7 @@ static int launch_impl(const SpmmArgs &a) {
       }
       for (int64_t fb = 0; fb < a.N; fb += 256) {  // one sweep per 256-feature tile, counter re-zeroed in between
         const int W = (int)(a.N - fb < 256 ? a.N - fb : 256);
-        if (fb && hipMemsetAsync(&hdr->arrivals, 0, sizeof(int), a.st) != hipSuccess) return DGS_ELAUNCH;
+        if (fb && fill_words(&hdr->arrivals, 0u, sizeof(int), a.st) != DGS_OK) return DGS_ELAUNCH;
         hipLaunchKernelGGL(kern, dim3((unsigned)P.nwg), dim3(kPanelBlock), P.lds, a.st, (int)a.M, W, (int)a.N, P.R, tl,
                            P.pcols, P.npanels, P.nsb, P.lead, a.rowptr, a.col, a.val, a.B + fb, a.C + fb,
                            a.E ? a.E + fb : nullptr, &hdr->arrivals,
@@ -1759,7 +1759,7 @@ static int launch_impl(const SpmmArgs &a) {
       ut.part_bytes = (unsigned)(L.max_pslots * ut.pstride * 4);
       ut.slot_long = reinterpret_cast<const int *>(pb + (a.plan_off_hub ? plan_off_slot((size_t)a.plan_off_hub, a.plan_hub) : PL.off_slot));
       ut.arrive = reinterpret_cast<int *>(w + L.off_arrive);
-      if (hipMemsetAsync(ut.arrive, 0, (size_t)a.plan_long * a.tiles * sizeof(int), a.st) != hipSuccess) return DGS_ELAUNCH;
+      if (fill_words(ut.arrive, 0u, (size_t)a.plan_long * a.tiles * sizeof(int), a.st) != DGS_OK) return DGS_ELAUNCH;
     }
     launch_fused<G, V, OP, HAS_VAL, ACC>(a, nbh, nbu, nbr, rpw, ut, part, parte, ha);
     if (a.plan_long > 0 && !fold) {
@@ -1778,7 +1778,7 @@ static int launch_impl(const SpmmArgs &a) {
   float *part = reinterpret_cast<float *>(w + L.off_part);
   int *parte = reinterpret_cast<int *>(w + L.off_parte);
   UnitTab ut{&hdr->n_units, &hdr->n_long, nullptr, units, longrows};
-  if (hipMemsetAsync(hdr, 0, sizeof(SpmmWs), a.st) != hipSuccess) return DGS_ELAUNCH;
+  if (fill_words(hdr, 0u, sizeof(SpmmWs), a.st) != DGS_OK) return DGS_ELAUNCH;
   const int64_t k0b = (a.M + (int64_t)kBlock * kK0Rows - 1) / ((int64_t)kBlock * kK0Rows);
   const int thub = hub_ok<OP, V, G, ACC>() ? hub_threshold(a.hints) : INT_MAX;
   const HubTab ht = hub_tab(a.nnz, thub < INT_MAX ? thub : kHubChainMin, a.nnz / kT1 + 2);
@@ -1816,7 +1816,7 @@ static int launch_impl(const SpmmArgs &a) {
 static inline bool strict_over_plan_ok() { return tuning().strict_mid == kTuneUnset && tuning().strict_hub == kTuneUnset; }
 
 #if defined(DGS_TU_STRICT)
-// Strict-order sum / mean (spmm_strict.h).  memset + classify_strict + ONE fused launch (no combine); dense graphs keep the
+// Strict-order sum / mean (spmm_strict.h).  fill + classify_strict + ONE fused launch (no combine); dense graphs keep the
 // column-panel sweep for rows up to tlong nnz (its per-row accumulator is a sequential fmaf chain already) and send only
 // the longer rows through strict unit waves.
 template <int G, int V, int OP, bool HAS_VAL, int STRICT>
@@ -1862,7 +1862,7 @@ static int launch_strict(const SpmmArgs &a) {
   if (thub < (strict_coop(G, V) ? kStrictMid : kStrictHub)) thub = strict_coop(G, V) ? kStrictMid : kStrictHub;
   if (tmid < kStrictMid) tmid = kStrictMid;
   if (tmid > thub) tmid = thub;
-  if (hipMemsetAsync(hdr, 0, sizeof(SpmmWs), a.st) != hipSuccess) return DGS_ELAUNCH;
+  if (fill_words(hdr, 0u, sizeof(SpmmWs), a.st) != DGS_OK) return DGS_ELAUNCH;
   const int64_t k0b = (a.M + (int64_t)kBlock * kK0Rows - 1) / ((int64_t)kBlock * kK0Rows);
   // unit blocks: first in the grid (the long chains must start first), twice as many as fit the chip at once (4 workgroups
   // per CU): the later ones take over as the early ones run out of units, and the row blocks follow as those drain.
@@ -1890,7 +1890,7 @@ static int launch_strict(const SpmmArgs &a) {
       }
       for (int64_t fb = 0; fb < a.N; fb += 256) {
         const int W = (int)(a.N - fb < 256 ? a.N - fb : 256);
-        if (fb && hipMemsetAsync(&hdr->arrivals, 0, sizeof(int), a.st) != hipSuccess) return DGS_ELAUNCH;
+        if (fb && fill_words(&hdr->arrivals, 0u, sizeof(int), a.st) != DGS_OK) return DGS_ELAUNCH;
         hipLaunchKernelGGL(kern, dim3((unsigned)P.nwg), dim3(kPanelBlock), P.lds, a.st, (int)a.M, W, (int)a.N, P.R, tl,
                            P.pcols, P.npanels, P.nsb, P.lead, a.rowptr, a.col, a.val, a.B + fb, a.C + fb,
                            (int *)nullptr, &hdr->arrivals, Epi{});

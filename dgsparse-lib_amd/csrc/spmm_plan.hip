@@ -26,7 +26,7 @@ namespace dgs {
 // the plan lists rows longer than kT1 as units while the fused kernel hands rows to the unit table from kT2: one threshold
 static_assert(kT1 == kT2, "spmm_plan.hip assumes DGS_T2 == DGS_T1 (rows in (T1, T2] would be computed twice)");
 
-struct PlanWs {  // build-time counters (zeroed by the first memset)
+struct PlanWs {  // build-time counters (zeroed by the first fill)
   int n_longlist;
   int n_hub;
   int pad[2];
@@ -423,15 +423,15 @@ extern "C" int dgs_spmm_plan_build2(int64_t M, int64_t K, int64_t nnz, const int
   // hub rows (dgs_common.h Tuning::hub_chain; spmm_impl.h hub_threshold): listed longest first for the sum / mean launches
   const int thub = plan_hub_threshold();
 
-  if (hipMemsetAsync(hdr, 0, PL.off_units, st) != hipSuccess) return DGS_ELAUNCH;
-  if (hipMemsetAsync(ws, 0, WL.off_list, st) != hipSuccess) return DGS_ELAUNCH;           // counters, cnt, cum
-  if (hipMemsetAsync(rinfo, 0, (size_t)WL.cap_long * 16, st) != hipSuccess) return DGS_ELAUNCH;
-  if (hipMemsetAsync(keys_in, 0xFF, (size_t)PL.max_units * 8, st) != hipSuccess) return DGS_ELAUNCH;  // unused = last
-  if (hipMemsetAsync(units_in, 0, (size_t)PL.max_units * 16, st) != hipSuccess) return DGS_ELAUNCH;
-  if (hipMemsetAsync(hkeys_in, 0xFF, (size_t)PL.max_hub * 4, st) != hipSuccess) return DGS_ELAUNCH;
-  if (hipMemsetAsync(hub_in, 0, (size_t)PL.max_hub * 16, st) != hipSuccess) return DGS_ELAUNCH;
-  if (hipMemsetAsync(skeys_in, 0xFF, (size_t)WL.cap_long * 4, st) != hipSuccess) return DGS_ELAUNCH;
-  if (hipMemsetAsync(srows_in, 0, (size_t)WL.cap_long * 16, st) != hipSuccess) return DGS_ELAUNCH;
+  if (fill_words(hdr, 0u, PL.off_units, st) != DGS_OK) return DGS_ELAUNCH;
+  if (fill_words(ws, 0u, WL.off_list, st) != DGS_OK) return DGS_ELAUNCH;           // counters, cnt, cum
+  if (fill_words(rinfo, 0u, (size_t)WL.cap_long * 16, st) != DGS_OK) return DGS_ELAUNCH;
+  if (fill_words(keys_in, 0xffffffffu, (size_t)PL.max_units * 8, st) != DGS_OK) return DGS_ELAUNCH;  // unused = last
+  if (fill_words(units_in, 0u, (size_t)PL.max_units * 16, st) != DGS_OK) return DGS_ELAUNCH;
+  if (fill_words(hkeys_in, 0xffffffffu, (size_t)PL.max_hub * 4, st) != DGS_OK) return DGS_ELAUNCH;
+  if (fill_words(hub_in, 0u, (size_t)PL.max_hub * 16, st) != DGS_OK) return DGS_ELAUNCH;
+  if (fill_words(skeys_in, 0xffffffffu, (size_t)WL.cap_long * 4, st) != DGS_OK) return DGS_ELAUNCH;
+  if (fill_words(srows_in, 0u, (size_t)WL.cap_long * 16, st) != DGS_OK) return DGS_ELAUNCH;
 
   size_t tb = WL.tmp_bytes;
   const int *prefix = col_prefix;

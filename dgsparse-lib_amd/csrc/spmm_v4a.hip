@@ -216,8 +216,8 @@ static void generate(const Shape &sh, const Layout &L, char *base, hipStream_t s
                      reinterpret_cast<float *>(base + L.val), reinterpret_cast<float *>(base + L.B));
 }
 static int product(const Shape &sh, const Layout &L, char *base, int op, int hints, float *C, int *E, hipStream_t st) {
-  if (hipMemsetAsync(C, 0xFF, (size_t)sh.M * sh.N * 4, st) != hipSuccess) return DGS_ELAUNCH;  // NaN: an unwritten element fails
-  if (E && hipMemsetAsync(E, 0x7F, (size_t)sh.M * sh.N * 4, st) != hipSuccess) return DGS_ELAUNCH;
+  if (fill_words(C, 0xffffffffu, (size_t)sh.M * sh.N * 4, st) != DGS_OK) return DGS_ELAUNCH;  // NaN: an unwritten element fails
+  if (E && fill_words(E, 0x7f7f7f7fu, (size_t)sh.M * sh.N * 4, st) != DGS_OK) return DGS_ELAUNCH;
   const FeatMap fm = feat_map(sh.N, true);
   SpmmArgs a{sh.M, sh.K, sh.N, sh.nnz(), reinterpret_cast<int *>(base + L.rowptr), reinterpret_cast<int *>(base + L.col),
              reinterpret_cast<float *>(base + L.val), reinterpret_cast<float *>(base + L.B), C, E, fm.tiles,
@@ -318,7 +318,7 @@ extern "C" int dgs_spmm_fold_selftest(void *scratch, size_t scratch_bytes, int r
   if (!scratch || scratch_bytes < dgs_spmm_hub_selftest_bytes() || !is_aligned16(scratch) || rounds < 1 || rounds > 1000) return DGS_EWORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   char *base = static_cast<char *>(scratch);
-  if (hipMemsetAsync(base, 0, 256, st) != hipSuccess) return DGS_ELAUNCH;
+  if (fill_words(base, 0u, 256, st) != DGS_OK) return DGS_ELAUNCH;
   hipStream_t ld = nullptr;
   hipEvent_t ev = nullptr;
   if (flags & 1) {
@@ -354,7 +354,7 @@ extern "C" int dgs_spmm_hub_selftest(void *scratch, size_t scratch_bytes, dgsStr
   char *base = static_cast<char *>(scratch);
   int verdict = 1;
   if (want_hub) {
-    if (hipMemsetAsync(base, 0, 256, st) != hipSuccess) return DGS_ELAUNCH;  // the mismatch counters
+    if (fill_words(base, 0u, 256, st) != DGS_OK) return DGS_ELAUNCH;  // the mismatch counters
     for (int h = 0; h < selftest::kNumHubShapes; h++) {
       const int rc = selftest::hub_shape(selftest::kHubShapes[h], h, base, st);  // (stream order: one shape's arrays are dead when the next one's are written)
       if (rc != DGS_OK) return rc;
@@ -391,7 +391,7 @@ extern "C" int dgs_spmm_csr_f32(int reduce_op, int64_t M, int64_t K, int64_t N, 
   if (!rowptr || !C || (nnz > 0 && (!col || !B)) || (arg && !E)) return DGS_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (E && !arg) {  // the reference leaves E = -1 for sum/mean (Eidx is never updated)
-    if (hipMemsetAsync(E, 0xFF, (size_t)M * N * sizeof(int32_t), st) != hipSuccess) return DGS_ELAUNCH;
+    if (fill_words(E, 0xffffffffu, (size_t)M * N * sizeof(int32_t), st) != DGS_OK) return DGS_ELAUNCH;
   }
   const size_t need = dgs_spmm_csr_workspace_bytes(reduce_op, M, N, nnz);
   if (need > 0 && (!workspace || workspace_bytes < need)) return DGS_EWORKSPACE;
@@ -418,7 +418,7 @@ extern "C" int dgs_spmm_csr_ex_f32(int reduce_op, int64_t M, int64_t K, int64_t 
   if (!rowptr || !C || (nnz > 0 && (!col || !B)) || (arg && !E)) return DGS_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (E && !arg) {
-    if (hipMemsetAsync(E, 0xFF, (size_t)M * N * sizeof(int32_t), st) != hipSuccess) return DGS_ELAUNCH;
+    if (fill_words(E, 0xffffffffu, (size_t)M * N * sizeof(int32_t), st) != DGS_OK) return DGS_ELAUNCH;
   }
   // (a strict call uses the plan's strict table unless an experiment override moved the class thresholds)
   const bool planned = plan && info && (!strict || strict_over_plan_ok()) && nnz > 0 && !tiny_problem(M, nnz) &&
@@ -459,7 +459,7 @@ extern "C" int dgs_spmm_csr_plan_f32(int reduce_op, int64_t M, int64_t K, int64_
   if (!rowptr || !C || !col || !B || (arg && !E)) return DGS_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (E && !arg) {
-    if (hipMemsetAsync(E, 0xFF, (size_t)M * N * sizeof(int32_t), st) != hipSuccess) return DGS_ELAUNCH;
+    if (fill_words(E, 0xffffffffu, (size_t)M * N * sizeof(int32_t), st) != DGS_OK) return DGS_ELAUNCH;
   }
   const size_t need = dgs_spmm_csr_plan_workspace_bytes(reduce_op, M, N, nnz, info);
   if (!workspace || workspace_bytes < need) return DGS_EWORKSPACE;
