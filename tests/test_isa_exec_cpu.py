@@ -3,7 +3,7 @@
 A divergent loop is left with an empty exec mask: the last lanes took themselves out of it, and the mask of the loop's entry is put back by the first
 instruction behind it (s_or_b64 exec, ...).  A vector instruction between the two does nothing.  The compiler has no reason to put one there, but
 its register allocator has: a spilled register that is reloaded "behind the loop" and lands in front of the instruction that puts the mask back.
-Every kernel with scratch memory is disassembled and searched for it; no GPU."""
+Every kernel that spills, to scratch memory or to accumulation registers, is disassembled and searched for it; no GPU."""
 import re
 import subprocess
 
@@ -37,7 +37,8 @@ def empty_reloads(code):
     index = {c[0]: i for i, c in enumerate(code)}
     starts = set()
     for i, (_, op, args, target) in enumerate(code):
-        if op == 's_cbranch_execz' and target in index:
+        # (a branch on a mask that nothing has narrowed just before is never taken: the compiler's way to fall through)
+        if op == 's_cbranch_execz' and target in index and any(writes_exec(c[1], c[2]) for c in code[max(i - 2, 0):i]):
             starts.add(index[target])
         if op == 's_cbranch_execnz' and i and code[i - 1][1] == 's_andn2_b64' and code[i - 1][2].startswith('exec'):
             starts.add(i + 1)
@@ -76,9 +77,12 @@ def test_the_search_finds_the_reload_and_nothing_else():
 
 def test_no_kernel_reloads_a_register_for_no_lane(kernels):  # noqa: F811
     by_object = {}
-    for name, k in kernels.items():
-        if k['scratch']:
-            by_object.setdefault(k['co'], []).append(name)
+    for co in sorted({k['co'] for k in kernels.values()}):
+        notes = subprocess.run([f'{LLVM}/llvm-readelf', '--notes', co], capture_output=True, text=True, check=True).stdout
+        for k in re.split(r'\n\s+- \.agpr_count:', notes)[1:]:
+            name = re.search(r'\.name:\s+(\S+)', k).group(1)
+            if int(re.match(r'\s*(\d+)', k).group(1)) or kernels[name]['scratch']:
+                by_object.setdefault(co, []).append(name)
     searched, bad = 0, {}
     for co, names in by_object.items():
         for at in range(0, len(names), 50):
@@ -93,5 +97,5 @@ def test_no_kernel_reloads_a_register_for_no_lane(kernels):  # noqa: F811
                 found = empty_reloads(code)
                 if found:
                     bad[kernels[m.group(1)]['demangled']] = found
-    assert searched == sum(len(n) for n in by_object.values()) and searched > 50, searched
+    assert searched == sum(len(n) for n in by_object.values()) and searched > 100, searched
     assert not bad, bad
