@@ -32,19 +32,6 @@ __device__ __forceinline__ void load_row(const T *p, int c, int D, float (&o)[kV
     for (int v = 0; v < V; v++) o[v] = c + v < D ? to_f32(p[c + v]) : 0.0f;
   }
 }
-// the same for data that this kernel reads once: non-temporal
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void load_row_stream(const T *p, int c, int D, float (&o)[kVec<T>]) {
-  constexpr int V = kVec<T>;
-  if constexpr (VECTOR) {
-    union { dgs_u4 u; T t[V]; } x;
-    x.u = __builtin_nontemporal_load(reinterpret_cast<const dgs_u4 *>(p + c));
-#pragma unroll
-    for (int v = 0; v < V; v++) o[v] = to_f32(x.t[v]);
-  } else {
-    load_row<T, VECTOR>(p, c, D, o);
-  }
-}
 template <typename T, bool VECTOR>
 __device__ __forceinline__ void store_row(T *p, int c, int D, const float (&o)[kVec<T>]) {
   constexpr int V = kVec<T>;
@@ -59,6 +46,7 @@ __device__ __forceinline__ void store_row(T *p, int c, int D, const float (&o)[k
       if (c + v < D) p[c + v] = from_f32<T>(o[v]);
   }
 }
+// the same past the caches: non-temporal
 template <typename T, bool VECTOR>
 __device__ __forceinline__ void store_row_stream(T *p, int c, int D, const float (&o)[kVec<T>]) {
   constexpr int V = kVec<T>;

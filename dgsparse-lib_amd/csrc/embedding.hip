@@ -2,7 +2,7 @@
 //
 //   out[p, :] = scale * table[ids[p], :]              a negative id is "no token": a row of zeros; an id >= V gives a row of NaN (nothing is
 //                                                     read out of bounds, and the mistake is seen)
-//   dtable[v, :] = scale * sum over p with ids[p] = v, in the order of p, of dout[p, :]       (ids that are negative, >= V or equal to the
+//   dtable[v, :] = scale * sum over p with ids[p] = v of dout[p, :], in a fixed order         (ids that are negative, >= V or equal to the
 //                                                     padding id add to no row; a row without a token is 0)
 //
 // Lookup: HBM-bound gather, each row read once in 16-byte pieces.

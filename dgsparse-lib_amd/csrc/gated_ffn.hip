@@ -390,8 +390,10 @@ static int launch_product(GemmArgs g, PlainOut o, const TilePlan &p, float *part
 }
 
 // Products that take gated_few_kernel.  Beyond 48 rows its reads of x out of L2 for every 16 columns cost more than the 64-row tiles' waste, if
-// those fill the card.  Few and tiles, us: 2048 x 5504 fp16: 32 rows 13.9 and 18.5, 48 rows 17.7 and 18.6, 64 rows 22.1 and 18.8;  64 x 4096 x 4096 bf16 (128
-// tiles) 20.9 and 33.7;  1024 x 4096 fp32: 48 rows 15.1 and 22.9, 64 rows 19.3 and 23.0.
+// those fill the card and the weights are in its last cache.  Few and tiles, us, called again on the same weights: 2048 x 5504 fp16: 32 rows 13.9 and
+// 18.5, 48 rows 17.7 and 18.6, 64 rows 22.1 and 18.8;  64 x 4096 x 4096 bf16 (128 tiles) 20.9 and 33.7;  1024 x 4096 fp32: 48 rows 15.1 and 22.9, 64 rows 19.3 and
+// 23.0.  On weights that come from memory, 64 rows, bf16: 4096 x 2048 24.9 and 50.8, 4096 x 4096 27.1 and 52.6, 4096 x 5504 47.2 and 52.3, 4096 x 8192 49.3 and
+// 52.9, 2048 x 4096 17.2 and 27.4, 2048 x 5504 27.4 and 28.4.
 template <typename T>
 static bool few_rows(int64_t rows, int64_t F) {
   return rows <= 48 || (rows <= 64 && (sizeof(T) == 4 || (F + 31) / 32 < cu_count() * 5 / 8));

@@ -166,7 +166,7 @@ struct Shares {
 };
 
 // The tile's sums: acc[i][j] = 16 x 16 at rows 16 i, columns col_of(j) of the wave's part; lane l register r holds m = l % 16, n = 4 (l / 16) + r.
-// STEP(i, j, part) is called for each 128 bytes of K where SCALED (8-bit types) instead of accumulating straight on.
+// (The 8-bit product keeps its own walk over K, with a scale behind each 128 bytes: fp8_kernel.)
 template <typename T, int BM, int BN, int WM, int WN, bool A_KO, bool B_KO, int PAIR>
 struct Gemm : Shares<BM, BN, WM, WN, PAIR> {
   using S = Shares<BM, BN, WM, WN, PAIR>;

@@ -267,8 +267,9 @@ FfnIn ffn_in(const Tensor &x_, const Tensor &wg_, const Tensor &wu_) {
 }
 // Whether the forward pass keeps the two products in 32 bits for the backward pass, where the caller leaves it open (keep < 0).  Kept they cost
 // 16 bytes of memory traffic for each value of h, made again 4 D flops.  rows x D x F, forward and backward, kept and made again, us, 32 bits:
-// 169343 x 128 x 512 1198 and 1176, 16384 x 160 x 1024 350 and 367, 30000 x 300 x 600 578 and 663, 4096 x 768 x 2048 580 and 712; 16 bits meet at D = 1024
-// (1.1 PFLOP/s against 5 TB/s).  Beyond 1 GiB of them they are made again, so that a deep model's activations stay its own.
+// 169343 x 128 x 512 1198 and 1176, 16384 x 160 x 1024 350 and 367, 30000 x 300 x 600 578 and 663, 4096 x 768 x 2048 580 and 712; bf16:
+// 32768 x 256 x 1024 369 and 303, 16384 x 512 x 2048 481 and 465, 16384 x 768 x 2816 754 and 753, 8192 x 1024 x 2816 473 and 507, 4096 x 2048 x 5504 672 and 757.
+// Beyond 1 GiB of them they are made again, so that a deep model's activations stay its own.
 bool ffn_keeps(const Tensor &x, const Tensor &wg, int64_t keep) {
   if (keep >= 0) return keep != 0;
   const int64_t D = x.size(-1), count = x.numel() / D * wg.size(0);

@@ -23,8 +23,8 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     the table's end is a mistake that costs no memory access: its row is NaN.  ``padding_idx`` names a row that is looked up like any
     other but gets no gradient.
 
-    Gradient of ``table``: every row is ``scale *`` the sum of the output's gradient over the places that hold its id, added up in the
-    order of the places (the same bits on every run), zero for rows without a place."""
+    Gradient of ``table``: every row is ``scale *`` the sum of the output's gradient over the places that hold its id, added up in a fixed
+    order (the same bits on every run), zero for rows without a place."""
     if padding_idx is not None and padding_idx < 0:
         raise ValueError('dgsparse: padding_idx must not be negative (negative ids are "no token" already)')
     return _embedding(ids, table, scale, -1 if padding_idx is None else padding_idx)

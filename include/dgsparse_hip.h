@@ -430,17 +430,18 @@ int dgs_spmm_min_merge_f32(int64_t R, int64_t N, const int32_t *rowmap, const in
  * Element type of a call's tensors.  Sums, row statistics and running values are held in 32 bits whatever the type; a result is rounded
  * to the type once, when it is stored.  Rows are contiguous (unit stride); `ld*` is the distance between rows in elements.  None of these
  * entries allocates, synchronises or keeps state; they may be recorded into a graph (no memset nodes).  All of them return DGS_EINVAL
- * for a null required pointer, a negative size or an unknown type, DGS_ERANGE for sizes beyond the indexing, DGS_EWORKSPACE for a
- * workspace that is too small. */
+ * for a null required pointer, a negative size or an unknown type, DGS_ERANGE for sizes beyond the indexing (rows of gated_ffn and of the 8-bit
+ * product: 256 of them within 2^31 bytes), DGS_EWORKSPACE for a workspace that is too small.  Outputs must not overlap inputs. */
 enum { DGS_F32 = 0, DGS_F16 = 1, DGS_BF16 = 2 };
 
 /* Embedding lookup: out[p, :] = scale * table[ids[p], :].  ids[n] of id_bytes = 4 | 8; table [V, D]; out [n, D] contiguous.  A negative id
  * stands for "no token": its row is 0.  An id >= V is a mistake: nothing is read for it and its row is NaN. */
 int dgs_embedding(int dtype, int id_bytes, int64_t n, int64_t V, int64_t D, const void *ids, const void *table, int64_t ld_table,
                   float scale, void *out, dgsStream_t stream);
-/* Its gradient: dtable[v, :] = scale * sum over p with ids[p] == v, in the order of p, of dout[p, :]; every row of dtable [V, D] is written.
+/* Its gradient: dtable[v, :] = scale * sum over p with ids[p] == v of dout[p, :], in a fixed order (32 or 64 neighbouring places of the sorted list at a
+ * time, in the order of p; then these sums); every row of dtable [V, D] is written.
  * Ids that are negative, >= V or equal to padding_idx (< 0: none) add to no row.  Deterministic: positions are sorted by id, no atomics
- * on values.  dout [n, D]; workspace dgs_embedding_bwd_workspace_bytes(), 256-byte aligned. */
+ * on values.  dout [n, D]; workspace dgs_embedding_bwd_workspace_bytes() (0 for sizes that the entry refuses), 256-byte aligned. */
 size_t dgs_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
 int dgs_embedding_bwd(int dtype, int id_bytes, int64_t n, int64_t V, int64_t D, const void *ids, int64_t padding_idx, const void *dout,
                       int64_t ld_dout, float scale, void *dtable, void *workspace, size_t workspace_bytes, dgsStream_t stream);
