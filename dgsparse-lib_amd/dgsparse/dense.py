@@ -80,5 +80,6 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     r"""``a @ b.T`` of 8-bit operands with a scale for each block of 128: ``a`` [..., K] with ``a_scale`` [..., ceil(K / 128)]
     (:func:`add_rms_norm_fp8`, ``quantize_fp8(x)``), ``b`` [N, K] with ``b_scale`` [ceil(N / 128), ceil(K / 128)] (``quantize_fp8(w, 128)``) ->
-    [..., N] in ``out_dtype``.  Sums in 32 bits, one rounding.  For serving: it records no gradient."""
+    [..., N] in ``out_dtype``.  Sums in 32 bits, one rounding; so is the product of a block's two scales, which has to lie in their normal range
+    (largest values of a row and of a block of weights whose product is between 2e-33 and 6e43).  For serving: it records no gradient."""
     return _matmul_fp8(a, a_scale, b, b_scale, out_dtype)

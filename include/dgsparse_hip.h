@@ -483,7 +483,7 @@ int dgs_gated_ffn_tiles(int dtype, int64_t rows, int64_t D, int64_t F, int32_t *
 int dgs_quantize_fp8(int dtype, int64_t rows, int64_t cols, const void *x, int64_t ldx, int block_rows, uint8_t *q, float *scales,
                      dgsStream_t stream);
 /* out [M, N] = A B^T of e4m3 operands: a [M, K] (row distance lda) with a_scale [M, ceil(K / 128)], b [N, K] (ldb) with b_scale
- * [ceil(N / 128), ceil(K / 128)], all scales contiguous; out contiguous, 16-byte aligned, rounded once to out_dtype.  Where K is a multiple of
+ * [ceil(N / 128), ceil(K / 128)], all scales contiguous; a block's two scales are multiplied in 32 bits; out contiguous, 16-byte aligned, rounded once to out_dtype.  Where K is a multiple of
  * 16, a and b have to lie at multiples of 16 bytes, their row distances too; any other K is taken through padded copies. */
 size_t dgs_matmul_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int dgs_matmul_fp8(int out_dtype, int64_t M, int64_t N, int64_t K, const uint8_t *a, int64_t lda, const float *a_scale, const uint8_t *b,
