@@ -19,6 +19,9 @@ static __global__ __launch_bounds__(kBlock) void fill_words_kernel(uint32_t *__r
 }
 int fill_words(void *p, uint32_t word, size_t bytes, hipStream_t st) {
   if (bytes == 0) return DGS_OK;
+#ifdef DGS_HOST_EMU  // (the emulation has no graphs, and its memset is the host's: words of four equal bytes)
+  return hipMemsetAsync(p, (int)(word & 0xff), bytes, st) == hipSuccess ? DGS_OK : DGS_ELAUNCH;
+#endif
   const int64_t words = (int64_t)(bytes / 4), pieces = is_aligned16(p) ? words / 4 : 0, work = pieces ? pieces : words;
   const int64_t blocks = (work + kBlock - 1) / kBlock;
   hipLaunchKernelGGL(fill_words_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(kBlock), 0, st, static_cast<uint32_t *>(p), word, words, pieces);

@@ -633,7 +633,6 @@ void block_sync() {
 // "name grid.x grid.y" line each - how the tests see WHICH kernels a C-ABI call took and how many launches it cost.
 static std::string g_launch_log;
 void log_launch(const char *kern, dim3 grid) {
-  if (!strcmp(kern, "fill_words_kernel")) return;  // clearing is not logged, as it was not when it was a memset
   if (g_launch_log.size() < (1u << 20)) g_launch_log += std::string(kern) + " " + std::to_string(grid.x) + " " + std::to_string(grid.y) + "\n";
 }
 }  // namespace emu
